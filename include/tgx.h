@@ -422,6 +422,76 @@ TGX_API int tgx_step_ragged(tgx_ctx* ctx, int n_entries, const int32_t* rows, co
 TGX_API int64_t tgx_context_size(const tgx_ctx* ctx);
 TGX_API int32_t tgx_num_layers(const tgx_ctx* ctx);
 
+/* ---- a cache held in 4 bits, and page copies, as operators on device buffers ----------------------
+ * What a context does with option "kv.bits" 4, for a host that keeps its own pages: the quantising append, the read that gives the values back, attention
+ * over the cache for single tokens and portions, and the copy that forks rows and compacts pools.  No context: a call takes a device ordinal and a stream of
+ * it (hipStream_t; NULL = the device's default stream), enqueues and returns; the caller's current device stays.  Nothing is allocated and nothing waits, so
+ * every call may be captured into a graph.  Buffers belong to the caller and are alive until the stream is past the call.  Calls are independent of each other and
+ * may come from several host threads.  A refused call enqueues nothing; tgx_op_last_error() has the reason (of the calling host thread).
+ *
+ * A page holds 128 tokens of all key / value heads of one layer, tgx_kv4_page_bytes(kv_heads, head_dim) bytes (kv_heads * head_dim * 144), the next page follows
+ * without a gap; its inside is the library's.  64 neighbouring channels of a token and head are a group of 16 levels lo + step * n (lo, step bfloat16):
+ *   lo = min x rounded down to bfloat16, step = max((max x - lo) * (1 / 15) rounded up to bfloat16, 2^-126), n = min(15, rint((x - lo) * (1 / step))),
+ * each operation rounded to 32 bits.  A group that holds a number that is not finite (or whose spread is not) reads as NaN.
+ * Page numbers in `table` that are not in [0, pages) count as pages without tokens: nothing is appended there, attention does not see them, they read as zeros. */
+typedef struct tgx_kv4_cache {
+  void* pool;            /* device, 16-byte aligned: the pages of one layer                                              */
+  int64_t pages;
+  const int32_t* table;  /* device [seqs][table_stride]: table_len page numbers a sequence, of its tokens 0-127, 128-255, ... */
+  int32_t table_stride;
+  int32_t table_len;     /* <= table_stride                                                                              */
+  int32_t seqs;
+  int32_t kv_heads;
+  int32_t head_dim;      /* 64 or 128                                                                                    */
+} tgx_kv4_cache;
+
+/* The tokens of a call, [tokens] of them in entries: entry e brings tokens offsets[e] .. offsets[e + 1] - 1 (offsets NULL: the one token e; tokens = entries) of
+ * sequence seq[e] (seq NULL: e), at positions start[e], start[e] + 1, ...  The arrays are read on the device when the call runs.  An entry brings at most
+ * max_count tokens (those behind are left out).  An entry whose sequence or offsets are out of range brings nothing.  Entries of one call have positions of their own.
+ * Tokens that no entry brings are left as they were, in every output. */
+typedef struct tgx_kv4_batch {
+  int32_t entries;       /* 0 .. 65535; 0: the call does nothing */
+  int32_t max_count;
+  int64_t tokens;
+  const int32_t* seq;
+  const int32_t* start;
+  const int32_t* offsets;
+} tgx_kv4_batch;
+
+/* [tokens][heads][head_dim] on the device: strides in elements, a head's channels lie together */
+typedef struct tgx_kv4_rows {
+  void* data;
+  int32_t dtype;         /* tgx_dtype */
+  int64_t token_stride;
+  int64_t head_stride;
+} tgx_kv4_rows;
+
+TGX_API int64_t tgx_kv4_page_bytes(int kv_heads, int head_dim);      /* -1: not a shape that is built */
+
+/* Keys and values of the batch's tokens into their pages (k and v of one dtype); a token with a negative position is left out.  The rest of a page stays as it is. */
+TGX_API int tgx_kv4_append(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream);
+
+/* The values that the pages hold for the batch's tokens, each rounded once to the dtype of k and v. */
+TGX_API int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream);
+
+/* out = softmax(scale q . k) v over the keys that a token sees: those of its sequence at positions 0 .. its own, with window > 0 only the last `window` of them.
+ * heads query heads, heads / kv_heads (1 .. 16) neighbours a key / value head; out has q's dtype.  A token that sees nothing (a negative position, pages without
+ * tokens) gets zeros.  k, v (both or neither): keys and values of the batch's tokens, appended first; entries that read what another entry of the same call appends
+ * are given with offsets.  max_keys: at least the last position + 1 of every entry; it sizes the work's division, a smaller one costs time only.
+ * workspace: tgx_kv4_attend_workspace bytes (of the same arguments; may be 0), 16-byte aligned, the call's own until the stream is past it. */
+TGX_API int64_t tgx_kv4_attend_workspace(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, int heads, int window, int64_t max_keys, int device);
+TGX_API int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* q, int heads, const tgx_kv4_rows* k, const tgx_kv4_rows* v, float scale, int window,
+                           int64_t max_keys, const tgx_kv4_rows* out, void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/* Pages between (or inside) paged pools, 4-bit or 16-bit: for every layer l and pair i, page to[i] of dst becomes page from[i] of src.  A page is page_bytes (a
+ * multiple of 16), a layer's pool starts l * src_stride / dst_stride bytes (multiples of 16) behind src / dst.  from, to: device [n]; a pair with a page outside
+ * of its pool is left out.  No page is read and written, or written twice, by one call. */
+TGX_API int tgx_copy_pages(const void* src, int64_t src_pages, int64_t src_stride, void* dst, int64_t dst_pages, int64_t dst_stride, int layers, int64_t page_bytes,
+                           const int32_t* from, const int32_t* to, int n, int device, void* stream);
+
+/* Why the calling host thread's last operator call was refused. */
+TGX_API const char* tgx_op_last_error(void);
+
 /* ---- diagnostics ------------------------------------------------------------------------- */
 
 /* Last error text for this context (or for tgx_create when ctx == NULL). */

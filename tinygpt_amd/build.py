@@ -24,12 +24,12 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvi
          ] + (["-mllvm", "-amdgpu-mfma-vgpr-form"] if os.environ.get("TGX_VGPR_FORM", "1") == "1" else [])
 
 
-TUS = ["abi", "decode", "attn", "sampler", "prefill", "prefill_f32", "skinny", "stack", "stack_few", "stack_rows", "stack_line", "stack_gqa", "stack_ssd", "stack_recblk"]     # csrc/<name>.hip, compiled in parallel (csrc/ctx.h lists what each holds)
+TUS = ["abi", "decode", "attn", "sampler", "prefill", "prefill_f32", "skinny", "stack", "stack_few", "stack_rows", "stack_line", "stack_gqa", "stack_ssd", "stack_recblk", "kv4"]     # csrc/<name>.hip, compiled in parallel (csrc/ctx.h lists what each holds)
 OBJDIR = os.path.join(LIBDIR, "obj")
 
 
 def _deps():
-    deps = [os.path.join(HERE, "..", "include", "tgx.h"), os.path.join(CSRC, "ctx.h"), os.path.join(CSRC, "stack.h"), os.path.join(CSRC, "prefill_plan.h"), os.path.join(CSRC, "line_plan.h")]
+    deps = [os.path.join(HERE, "..", "include", "tgx.h"), os.path.join(CSRC, "ctx.h"), os.path.join(CSRC, "stack.h"), os.path.join(CSRC, "prefill_plan.h"), os.path.join(CSRC, "line_plan.h"), os.path.join(CSRC, "kv4_plan.h")]
     kd = os.path.join(CSRC, "kernels")
     return deps + [os.path.join(kd, f) for f in sorted(os.listdir(kd))]
 

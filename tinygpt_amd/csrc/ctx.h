@@ -9,6 +9,7 @@
 //   stack.hip        layered models (tgx_create_stack): ragged engine step, paged latent / key-value cache, slot state (kernels/stack*.h)
 //   stack_gqa.hip    their grouped-query attention on the matrix cores (kernels/stack_gqa_mfma.h)
 //   stack_ssd.hip    their blocked state-space recurrence on the matrix cores (kernels/stack_ssd_mfma.h)
+//   kv4.hip          the cache held in 4 bits and page copies: a context's launches, the operators on device buffers (kernels/kv4.h)
 // One context = one GPU = one HIP stream; every call comes from one host thread.  There is NO CPU path in this library.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -298,7 +299,7 @@ int dev_alloc(tgx_ctx* c, T** p, size_t n) {
   return TGX_OK;
 }
 
-namespace tgx { struct AttnArgs; struct FinalizeArgs; struct AttnPrefillArgs; struct RopeKvArgs; }
+namespace tgx { struct AttnArgs; struct FinalizeArgs; struct AttnPrefillArgs; struct RopeKvArgs; struct Kv4Args; struct Kv4Plan; struct CopyPagesArgs; }
 
 // ---- abi.hip
 void drop_step_graphs(tgx_ctx* c);
@@ -347,3 +348,8 @@ int ensure_skinny_ws(tgx_ctx* c, int rows);
 void launch_decode_step_mfma(tgx_ctx* c, int row0, int M, const tgx_sampler_cfg& cfg);
 void launch_prefill_skinny(tgx_ctx* c, int row0, int NB, int S);
 int skinny_set_attrs(tgx_ctx* c);
+// ---- kv4.hip (kernels/kv4.h)
+void kv4_launch_append(const tgx::Kv4Args& a, int hd, hipStream_t s);
+void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s);
+void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws, hipStream_t s);
+void launch_copy_pages(const tgx::CopyPagesArgs& a, int layers, hipStream_t s);

@@ -1,0 +1,631 @@
+// kv4.h — a key / value cache held in 4 bits: the append that fills its pages, the read that gives the values back, attention over it, page copies.
+//
+// Format.  64 neighbouring channels of a token and head are a group: 16 levels lo + step n.
+//   lo = bf16(min x, rounded down), step = max(bf16(f32((max x - lo) * (1 / 15)), rounded up), 2^-126), n = min(15, rint(f32(f32(x - lo) * f32(1 / step))))
+// every operation one IEEE f32 operation, so that the codes follow from the inputs alone, whichever kernel writes them.  Rounding lo down and step up keeps
+// every x inside the levels; x is off by half a step at most.  A group with a value that is not finite (or whose spread is not) is stored as lo = NaN, step = 0:
+// its values read as NaN, they do not pass for numbers.  4.5 bits a channel; a group of 64 is one MFMA's 32 channels twice, so that a score's factors stay
+// outside of the products (below).
+//
+// Layout.  A page holds KV_BLOCK = 128 tokens: [kv_heads][4 blocks of 32 tokens][36 HD bytes].  A block: key codes (16 HD bytes), value codes (16 HD), parameters
+// (4 HD).  The codes lie in the order in which the matrix cores take them as operands, eight to a 32-bit word, so that a lane's 16-byte load is its operand and
+// nothing passes through LDS: word (part * 64 + lane) * 4 + w, lane = 16 q + r, i = 4 part + w,
+//   keys    token 16 (i / (HD / 32)) + r, channels 32 (i % (HD / 32)) + 8 q + e        (the A operand of a 16 x 16 x 32 product: rows tokens)
+//   values  channel 16 i + r, token 4 q + e (e < 4) or 16 + 4 q + e - 4                 (the B operand, its contraction in the order in which the scores' lanes hold the tokens)
+// e = 0 .. 7 at bit 4 (e / 2 + 4 (e % 2)): (w >> 4 i) & 0x000f000f | 0x43004300 is the pair (2 i, 2 i + 1) as bf16 128 + n, exactly.
+// Parameters: [32 tokens][keys, values][HD / 64] words, lo in the low half, step in the high.
+#pragma once
+#include "common.h"
+#include "../kv4_plan.h"
+
+namespace tgx {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+
+template <int HD> constexpr int kv4_block_words() { return 9 * HD; }
+static_assert(KV4_PAGE == KV_BLOCK, "a page of the 4-bit cache holds as many tokens as one of the 16-bit cache");
+
+__device__ __forceinline__ float kv4_load(const void* p, long long i, int dt) {
+  if (dt == DT_F32) return static_cast<const float*>(p)[i];
+  const unsigned short u = static_cast<const unsigned short*>(p)[i];
+  return dt == DT_BF16 ? bf16_to_f32(u) : f16_bits_to_f32(u);
+}
+__device__ __forceinline__ void kv4_store(void* p, long long i, float v, int dt) {
+  if (dt == DT_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<unsigned short*>(p)[i] = dt == DT_BF16 ? f32_to_bf16(v) : f32_to_f16_bits(v);
+}
+
+// ---- one group's levels ----------------------------------------------------------------------------------------------------------------------------
+struct Kv4Levels { float lo, inv; unsigned int word; };       // word: the group's parameter word
+__device__ __forceinline__ Kv4Levels kv4_levels(float mn, float mx, bool bad) {
+  Kv4Levels g;
+  const unsigned int lb = __float_as_uint(mn);
+  g.lo = __uint_as_float((mn < 0.f ? lb + 0xffffu : lb) & 0xffff0000u);
+  const float spread = __fsub_rn(mx, g.lo);
+  const float step = fmaxf(__uint_as_float((__float_as_uint(__fmul_rn(spread, 1.0f / 15.0f)) + 0xffffu) & 0xffff0000u), 1.17549435e-38f);
+  g.inv = __fdiv_rn(1.0f, step);
+  if (bad || !(spread <= 3.402823466e38f)) { g.inv = 0.f; g.lo = 0.f; g.word = 0x00007fc0u; }      // codes 0, lo NaN, step 0
+  else g.word = (__float_as_uint(g.lo) >> 16) | __float_as_uint(step);
+  return g;
+}
+// a value that is not finite only meets a group that is stored as NaN: its codes are 0
+__device__ __forceinline__ unsigned int kv4_code(float x, const Kv4Levels& g) {
+  const float n = rintf(__fmul_rn(__fsub_rn(x, g.lo), g.inv));
+  return n > 0.f ? (unsigned int)fminf(n, 15.f) : 0u;      // (a NaN is not above 0)
+}
+__device__ __forceinline__ bool kv4_not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+// minimum / maximum over 32 neighbouring lanes, every lane gets it
+template <bool MAX> __device__ __forceinline__ float kv4_extreme32(float v) {
+  auto f = [](float x, float y) { return MAX ? fmaxf(x, y) : fminf(x, y); };
+  v = f(v, dpp_mov<0xB1, 0xf>(v));
+  v = f(v, dpp_mov<0x4E, 0xf>(v));
+  v = f(v, dpp_mov<0x141, 0xf>(v));
+  v = f(v, dpp_mov<0x140, 0xf>(v));
+  const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// One token of one kv head by one wave: a lane takes two channels (HD 64: lanes 0-31 the key, 32-63 the value; HD 128: the key, then the value), a group is 32
+// lanes.  A value word holds seven other tokens' codes, which stay: OWNED = nothing else writes the word in this launch, and it is read and stored; otherwise the
+// eight codes of a word may come from several entries and the change goes in by an atomic exclusive or, whose result does not depend on the order.
+template <int HD, bool OWNED>
+__device__ __forceinline__ void kv4_append_one(const Kv4Args& a, unsigned int* page, long long tok, int pos, int kvh) {
+  constexpr int ROUNDS = HD / 64;
+  const int lane = threadIdx.x & 63;
+  const int t = pos & (KV4_BLK - 1);
+  unsigned int* blk = page + (size_t)((pos >> 5) & 3) * kv4_block_words<HD>();
+  const long long slot = (long long)(pos & (KV_BLOCK - 1)) * a.slot_s;
+  float x[ROUNDS][2];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; r++) {
+    const bool val = HD == 64 ? lane >= 32 : r == 1;
+    const int ch = HD == 64 ? 2 * (lane & 31) : 2 * lane;
+    const long long at = val ? tok * a.v_ts + kvh * a.v_hs + slot + ch : tok * a.k_ts + kvh * a.k_hs + slot + ch;
+    const void* src = val ? a.v : a.k;
+    x[r][0] = kv4_load(src, at, a.kv_dt);
+    x[r][1] = kv4_load(src, at + 1, a.kv_dt);
+  }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; r++) {
+    const bool val = HD == 64 ? lane >= 32 : r == 1;
+    const int ch = HD == 64 ? 2 * (lane & 31) : 2 * lane, g = ch >> 6;
+    const float bad = kv4_extreme32<true>(kv4_not_finite(x[r][0]) || kv4_not_finite(x[r][1]) ? 1.f : 0.f);
+    const Kv4Levels lv = kv4_levels(kv4_extreme32<false>(fminf(x[r][0], x[r][1])), kv4_extreme32<true>(fmaxf(x[r][0], x[r][1])), bad != 0.f);
+    const unsigned int n0 = kv4_code(x[r][0], lv), n1 = kv4_code(x[r][1], lv);
+    if ((lane & 31) == 0) blk[kv4_param_word(HD, t, val ? 1 : 0, g)] = lv.word;
+    // a key word: eight channels = four lanes
+    const int i4 = 4 * (lane & 3);
+    int kw = (int)((n0 << i4) | (n1 << (i4 + 16)));
+    kw |= __builtin_amdgcn_update_dpp(0, kw, 0xB1, 0xf, 0xf, false);
+    kw |= __builtin_amdgcn_update_dpp(0, kw, 0x4E, 0xf, 0xf, false);
+    if (!val) {
+      if ((lane & 3) == 0) blk[kv4_key_word(HD, t, ch)] = (unsigned int)kw;
+    } else {
+      const int bit = kv4_value_bit(t);
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        unsigned int* w = blk + kv4_value_word(HD, t, ch + c);
+        const unsigned int n = (c ? n1 : n0) << bit, m = 15u << bit;
+        if constexpr (OWNED) *w = (*w & ~m) | n;
+        else {
+          const unsigned int old = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_fetch_xor(w, (old ^ n) & m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+    }
+  }
+}
+
+// Single tokens: a wave a (entry, kv head).
+template <int HD>
+__global__ __launch_bounds__(64) void kv4_append_token_kernel(const Kv4Args a) {
+  const Kv4Entry en = kv4_entry(a, blockIdx.y);
+  if (en.count < 1 || en.start < 0) return;
+  unsigned int* page = kv4_page(a, en.seq, en.start >> KV_BLOCK_SHIFT, blockIdx.x, HD);
+  if (page) kv4_append_one<HD, false>(a, page, en.tok0, en.start, blockIdx.x);
+}
+
+// Portions: a wave a (entry, block of 32 positions, kv head).  A lane takes a whole group of one token (32 tokens x HD / 64 groups x {key, value}): the levels need no
+// exchange.  The codes pass through LDS as bytes [token][channel], where a value word finds its eight tokens.
+template <int HD, int DT>
+__global__ __launch_bounds__(64) void kv4_append_block_kernel(const Kv4Args a) {
+  constexpr int G = HD / 64, LS = HD / 4 + 1;                  // LDS row of a token in words
+  __shared__ unsigned int s[KV4_BLK * LS];
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  const int kvh = blockIdx.x, lane = threadIdx.x;
+  if (en.count < 1) return;
+  const int s0 = max(en.start, 0), b = (s0 >> 5) + blockIdx.y;      // block of positions
+  const int p0 = max(s0, b * KV4_BLK), p1 = min(en.start + en.count, (b + 1) * KV4_BLK);
+  if (p0 >= p1) return;
+  unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
+  if (!page) return;
+  unsigned int* blk = page + (size_t)(b & 3) * kv4_block_words<HD>();
+#pragma unroll
+  for (int r = 0; r < G; r++) {
+    const int item = r * 64 + lane, val = item / (32 * G), rest = item % (32 * G), t = rest / G, g = rest % G, pos = b * KV4_BLK + t;
+    const bool in = pos >= p0 && pos < p1;
+    const long long tok = en.tok0 + (in ? pos - en.start : p0 - en.start);      // (a lane without a token reads one that is there)
+    const int sp = in ? pos : p0;
+    const elem_t<DT>* src = static_cast<const elem_t<DT>*>(val ? a.v : a.k) + (val ? tok * a.v_ts + kvh * a.v_hs : tok * a.k_ts + kvh * a.k_hs) + (long long)(sp & (KV_BLOCK - 1)) * a.slot_s + g * 64;
+    float x[64];
+    const bool wide = ((reinterpret_cast<uintptr_t>(src) & 15) == 0);
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) slice_unpack<DT>(load_slice<DT>(src, i), x + 8 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 64; i++) x[i] = elem_to_f32<DT>(src[i]);
+    }
+    float mn = x[0], mx = x[0];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 64; i++) { mn = fminf(mn, x[i]); mx = fmaxf(mx, x[i]); bad |= kv4_not_finite(x[i]); }
+    const Kv4Levels lv = kv4_levels(mn, mx, bad);
+    if (in) blk[kv4_param_word(HD, t, val, g)] = lv.word;
+    if (!val) {
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          unsigned int w = 0;
+#pragma unroll
+          for (int e = 0; e < 8; e++) w |= kv4_code(x[32 * c + 8 * q + e], lv) << kv4_code_bit(e);
+          if (in) blk[kv4_key_word(HD, t, 64 * g + 32 * c + 8 * q)] = w;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        unsigned int w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w |= kv4_code(x[4 * i + e], lv) << (8 * e);
+        s[t * LS + g * 16 + i] = w;
+      }
+    }
+  }
+  __syncthreads();
+  // value words: a lane takes four neighbouring channels of a quarter's eight tokens
+#pragma unroll
+  for (int u = 0; u < HD / 64; u++) {
+    const int item = u * 64 + lane, q = item / (HD / 4), c4 = item % (HD / 4);
+    unsigned int w[4] = {0, 0, 0, 0}, m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int t = kv4_value_token(q, e), pos = b * KV4_BLK + t, bit = kv4_code_bit(e);
+      const unsigned int cs = s[t * LS + c4];
+      if (pos >= p0 && pos < p1) {
+        m |= 15u << bit;
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[c] |= ((cs >> (8 * c)) & 15u) << bit;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      unsigned int* dst = blk + kv4_value_word(HD, 4 * q, 4 * c4 + c);
+      if (m == 0xffffffffu) *dst = w[c];
+      else if (m) {
+        const unsigned int old = __hip_atomic_load(dst, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_xor(dst, (old ^ w[c]) & m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+  }
+}
+
+// The values that the pages hold for the batch's tokens: a wave a (entry, block of 32 positions, kv head).
+template <int HD, int DT>
+__global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
+  constexpr int PARTS = HD / 64;
+  __shared__ unsigned char s[KV4_BLK * (HD + 8)];
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  const int kvh = blockIdx.x, lane = threadIdx.x, q = lane >> 4, r = lane & 15;
+  if (en.count < 1) return;
+  const int s0 = max(en.start, 0), b = (s0 >> 5) + blockIdx.y;
+  const int p0 = max(s0, b * KV4_BLK), p1 = min(en.start + en.count, (b + 1) * KV4_BLK);
+  if (p0 >= p1) return;
+  const unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
+  elem_t<DT>* ko = static_cast<elem_t<DT>*>(a.k);
+  elem_t<DT>* vo = static_cast<elem_t<DT>*>(a.v);
+  if (!page) {      // tokens without a page read as zeros
+    for (int p = p0; p < p1; p++)
+      for (int c = lane; c < HD; c += 64) {
+        const long long tok = en.tok0 + p - en.start;
+        ko[tok * a.k_ts + kvh * a.k_hs + c] = 0;
+        vo[tok * a.v_ts + kvh * a.v_hs + c] = 0;
+      }
+    return;
+  }
+  const unsigned int* blk = page + (size_t)(b & 3) * kv4_block_words<HD>();
+#pragma unroll
+  for (int p = 0; p < PARTS; p++) {
+    const u32x4 w = reinterpret_cast<const u32x4*>(blk)[p * 64 + lane], vw = reinterpret_cast<const u32x4*>(blk + 4 * HD)[p * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int i = 4 * p + j, t = 16 * (i / (HD / 32)) + r, chunk = i % (HD / 32), pos = b * KV4_BLK + t;
+      if (pos >= p0 && pos < p1) {
+        const unsigned int par = blk[kv4_param_word(HD, t, 0, chunk >> 1)];
+        const float lo = bf16_lo(par), st = bf16_hi(par);
+        elem_t<DT>* dst = ko + (en.tok0 + pos - en.start) * a.k_ts + kvh * a.k_hs + 32 * chunk + 8 * q;
+#pragma unroll
+        for (int e = 0; e < 8; e++) dst[e] = f32_to_elem<DT>(fmaf(st, (float)((w[j] >> kv4_code_bit(e)) & 15u), lo));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[kv4_value_token(q, e) * (HD + 8) + 16 * i + r] = (unsigned char)((vw[j] >> kv4_code_bit(e)) & 15u);
+    }
+  }
+  __syncthreads();
+  for (int item = lane; item < KV4_BLK * HD / 8; item += 64) {
+    const int t = item / (HD / 8), c8 = item % (HD / 8), pos = b * KV4_BLK + t;
+    if (pos < p0 || pos >= p1) continue;
+    const unsigned int par = blk[kv4_param_word(HD, t, 1, c8 >> 3)];
+    const float lo = bf16_lo(par), st = bf16_hi(par);
+    elem_t<DT>* dst = vo + (en.tok0 + pos - en.start) * a.v_ts + kvh * a.v_hs + 8 * c8;
+    const u32x2 cs = *reinterpret_cast<const u32x2*>(s + t * (HD + 8) + 8 * c8);
+#pragma unroll
+    for (int e = 0; e < 8; e++) dst[e] = f32_to_elem<DT>(fmaf(st, (float)((cs[e >> 2] >> (8 * (e & 3))) & 255u), lo));
+  }
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------------------------------------------
+// S^T = K Q^T with the codes as the operand: a score is sum_g step_g (q_g . (128 + n_g)) + (lo_g - 128 step_g) sum(q_g), so that a product of 16 tokens x 16 query
+// columns (column = token of the entry, query head of the kv head) costs two fused multiply-adds a score and group and no value is unpacked.  O = P V the same
+// way: the weights p step_g (bf16, TERMS of them) meet 128 + n; what the 128 adds is taken off with the weights' own sum (a product with ones: the same rounded
+// weights), the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A operand
+// of P V, whose contraction runs over the tokens in the order of the value words.
+// TERMS: 16-bit terms of a query and of a weight.  Two keep what 32-bit inputs bring (2^-17); queries in bf16 are one term exactly.
+// KW = 4: the waves of a workgroup divide the keys (wave w: block w of every page), all columns in each; their sums meet in LDS.  KW = 1: they divide the
+// columns and walk the same keys.
+__device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
+  u32x4 f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  return __builtin_bit_cast(bf16x8_t, f);
+}
+__device__ __forceinline__ float kv4_max_quarters(float v) {      // over the lanes of equal r
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float kv4_sum_quarters(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <int HD, int NT, int KW, int TERMS>
+__global__ __launch_bounds__(256) void kv4_attend_kernel(const Kv4Args a) {
+  constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q4 = lane >> 4, r16 = lane & 15;
+  const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  const int ncol = en.count * a.group;
+  const int col0 = (KW == 4 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wv) * 16 * NT;
+  if (col0 >= ncol) return;      // (KW 1 has no barrier)
+  // this token's key and value first, by the workgroup whose pages hold its place (single tokens)
+  int my_pos[NT];
+  bool valid[NT];
+  const int first = en.start + min(col0, ncol - 1) / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;      // positions of the columns
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int c = col0 + 16 * t + r16;
+    valid[t] = c < ncol;
+    my_pos[t] = valid[t] ? en.start + c / a.group : -1;
+  }
+  // queries: column r, channels 32 c + 8 q .. + 7
+  bf16x8_t qf[NT][CH][TERMS];
+  float qsum[NT][G];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int c = min(col0 + 16 * t + r16, ncol - 1), i = c / a.group, h = kvh * a.group + c % a.group;
+    const long long base = (en.tok0 + i) * a.q_ts + h * a.q_hs + 8 * q4;
+#pragma unroll
+    for (int g = 0; g < G; g++) qsum[t][g] = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < CH; ch++) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = kv4_load(a.q, base + 32 * ch + e, a.q_dt);
+      bf16_t hi[8], lo[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        split16<DT_BF16>(x[e], hi[e], lo[e]);
+        qsum[t][ch / 2] += TERMS == 2 ? bf16_to_f32(hi[e]) + bf16_to_f32(lo[e]) : bf16_to_f32(hi[e]);
+      }
+      u32x4 f, fl;
+#pragma unroll
+      for (int e = 0; e < 4; e++) { f[e] = hi[2 * e] | ((unsigned)hi[2 * e + 1] << 16); fl[e] = lo[2 * e] | ((unsigned)lo[2 * e + 1] << 16); }
+      qf[t][ch][0] = __builtin_bit_cast(bf16x8_t, f);
+      if constexpr (TERMS == 2) qf[t][ch][1] = __builtin_bit_cast(bf16x8_t, fl);
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) qsum[t][g] = kv4_sum_quarters(qsum[t][g]);
+  }
+  f32x4 o[NT][CT], ones[NT][G];
+  float m[NT], l[NT], lov[NT][G];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) { lov[t][g] = 0.f; ones[t][g] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+#pragma unroll
+    for (int c = 0; c < CT; c++) o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  const int key_hi = last + 1, key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;      // keys that some column sees
+  const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
+  const int pg0 = rg.lo, pg1 = rg.hi;
+  if (KW == 4 && NT == 1 && a.k != nullptr && en.count == 1 && en.start >= 0) {
+    const int b = en.start >> KV_BLOCK_SHIFT;
+    if (b >= pg0 && b < pg1) {
+      unsigned int* page = kv4_page(a, en.seq, b, kvh, HD);
+      if (page && wv == 0) kv4_append_one<HD, true>(a, page, en.tok0, en.start, kvh);
+      __syncthreads();
+    }
+  }
+  for (int pg = pg0; pg < pg1; pg++) {
+    const unsigned int* page = kv4_page(a, en.seq, pg, kvh, HD);
+    if (!page) continue;
+#pragma unroll 1
+    for (int b = KW == 4 ? wv : 0; b < (KW == 4 ? wv + 1 : 4); b++) {
+      const int t0 = pg * KV_BLOCK + b * KV4_BLK;
+      if (t0 >= key_hi || t0 + KV4_BLK <= key_lo) continue;
+      const unsigned int* blk = page + (size_t)b * kv4_block_words<HD>();
+      u32x4 kw[PARTS], vw[PARTS], pw[2][2 * G];
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) kw[p] = reinterpret_cast<const u32x4*>(blk)[p * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2 * G; j++) pw[i][j] = reinterpret_cast<const u32x4*>(blk + 8 * HD + (16 * i + 4 * q4) * 2 * G)[j];
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) vw[p] = reinterpret_cast<const u32x4*>(blk + 4 * HD)[p * 64 + lane];
+      auto par = [&](int i, int r, int kv, int g) -> unsigned int { const int x = (r * 2 + kv) * G + g; return pw[i][x >> 2][x & 3]; };
+      const bool whole = t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window);      // every column sees every token of the block
+      // scores
+      f32x4 sc[NT][2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) sc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          bf16x8_t kf[2];
+#pragma unroll
+          for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(kw[x >> 2][x & 3]); }
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+              for (int term = 0; term < TERMS; term++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], qf[t][2 * g + c][term], d, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const unsigned int w = par(i, r, 0, g);
+              const float st = bf16_hi(w), z = fmaf(-128.f, st, bf16_lo(w));
+              sc[t][i][r] = fmaf(st, d[r], fmaf(z, qsum[t][g], sc[t][i][r]));
+            }
+          }
+        }
+      }
+      // weights
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float mx = -INFINITY;
+        bool seen[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int j = t0 + 16 * i + 4 * q4 + r;
+            seen[i][r] = whole || (j <= my_pos[t] && (a.window <= 0 || j > my_pos[t] - a.window));
+            sc[t][i][r] *= a.scale_log2;
+            if (!seen[i][r]) sc[t][i][r] = -INFINITY;
+            mx = fmaxf(mx, sc[t][i][r]);
+          }
+        mx = kv4_max_quarters(mx);
+        // the sums keep their reference until a maximum passes it by 8 (weights up to 256 then): few blocks rescale
+        if (__any(mx > m[t] + 8.f)) {
+          const float nm = fmaxf(m[t], mx), f = nm > m[t] ? __builtin_amdgcn_exp2f(m[t] - nm) : 1.f;
+          m[t] = nm;
+          l[t] *= f;
+#pragma unroll
+          for (int g = 0; g < G; g++) lov[t][g] *= f;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float fr = __shfl(f, 4 * q4 + r, 64);
+#pragma unroll
+            for (int c = 0; c < CT; c++) o[t][c][r] *= fr;
+#pragma unroll
+            for (int g = 0; g < G; g++) ones[t][g][r] *= fr;
+          }
+        }
+        float p[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            p[i][r] = seen[i][r] ? __builtin_amdgcn_exp2f(sc[t][i][r] - m[t]) : 0.f;
+            l[t] += p[i][r];
+          }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          float ps[8];
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const unsigned int w = par(i, r, 1, g);
+              ps[4 * i + r] = seen[i][r] ? p[i][r] * bf16_hi(w) : 0.f;
+              lov[t][g] = seen[i][r] ? fmaf(p[i][r], bf16_lo(w), lov[t][g]) : lov[t][g];
+            }
+          u32x4 pf, pl;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            pf[e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
+            if constexpr (TERMS == 2) pl[e] = pack_bf16(ps[2 * e] - bf16_lo(pf[e]), ps[2 * e + 1] - bf16_hi(pf[e]));
+          }
+          const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, pf), pq = __builtin_bit_cast(bf16x8_t, pl);
+          ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ph, one8, ones[t][g], 0, 0, 0);
+          if constexpr (TERMS == 2) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pq, one8, ones[t][g], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int x = 4 * g + c;
+            const bf16x8_t vf = kv4_frag(vw[x >> 2][x & 3]);
+            o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ph, vf, o[t][x], 0, 0, 0);
+            if constexpr (TERMS == 2) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pq, vf, o[t][x], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+  // the columns' sums: o - 128 sum(weights) + lo part, denominators over the four quarters
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    l[t] = kv4_sum_quarters(l[t]);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const float lg = kv4_sum_quarters(lov[t][g]);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float add = fmaf(-128.f, ones[t][g][r], __shfl(lg, 4 * q4 + r, 64));
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
+      }
+    }
+  }
+  if constexpr (KW == 4) {
+    // the four waves' sums meet two and two: a lane's registers are the same places in every wave
+    __shared__ float so[2][NT][CT * 4][64], sm[2][NT][2][64];
+#pragma unroll
+    for (int half = 2; half > 0; half >>= 1) {
+      __syncthreads();
+      if (wv >= half && wv < 2 * half) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          sm[wv - half][t][0][lane] = m[t]; sm[wv - half][t][1][lane] = l[t];
+#pragma unroll
+          for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) so[wv - half][t][c * 4 + r][lane] = o[t][c][r];
+        }
+      }
+      __syncthreads();
+      if (wv < half) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const float m2 = sm[wv][t][0][lane], l2 = sm[wv][t][1][lane], nm = fmaxf(m[t], m2);
+          const float f1 = m[t] == nm ? 1.f : __builtin_amdgcn_exp2f(m[t] - nm), f2 = m2 == nm ? 1.f : __builtin_amdgcn_exp2f(m2 - nm);      // (both -inf: sums of zero)
+          m[t] = nm;
+          l[t] = l[t] * f1 + l2 * f2;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float a1 = __shfl(f1, 4 * q4 + r, 64), a2 = __shfl(f2, 4 * q4 + r, 64);
+#pragma unroll
+            for (int c = 0; c < CT; c++) o[t][c][r] = o[t][c][r] * a1 + so[wv][t][c * 4 + r][lane] * a2;
+          }
+        }
+      }
+    }
+    if (wv != 0) return;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    if (a.splits > 1 && valid[t] && q4 == 0) {
+      const int c = col0 + 16 * t + r16;
+      const long long row = (en.tok0 + c / a.group) * a.heads + kvh * a.group + c % a.group;
+      a.ml[(row * a.splits + split) * 2] = m[t];
+      a.ml[(row * a.splits + split) * 2 + 1] = l[t];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int c = col0 + 16 * t + 4 * q4 + r;
+      const float den = __shfl(l[t], 4 * q4 + r, 64);
+      if (c >= ncol) continue;
+      const int i = c / a.group, h = kvh * a.group + c % a.group;
+      if (a.splits > 1) {
+        float* dst = a.part + (((en.tok0 + i) * a.heads + h) * a.splits + split) * HD;
+#pragma unroll
+        for (int x = 0; x < CT; x++) dst[16 * x + r16] = o[t][x][r];
+      } else {
+        const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
+        const long long at = (en.tok0 + i) * a.o_ts + h * a.o_hs;
+#pragma unroll
+        for (int x = 0; x < CT; x++) kv4_store(a.out, at + 16 * x + r16, round_storage_mode(o[t][x][r] * inv, a.act16), a.q_dt);
+      }
+    }
+  }
+}
+
+// The splits' records of a row (token, query head): a workgroup a row.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
+  constexpr int LN = HD / 4, WAYS = 256 / LN;                 // lanes of a row, splits at a time
+  __shared__ float sw[1024];
+  __shared__ f32x4 sacc[256];
+  __shared__ float stot;
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  if ((int)blockIdx.y >= en.count) return;
+  const int h = blockIdx.x, S = a.splits, tid = threadIdx.x;
+  const long long row = (en.tok0 + blockIdx.y) * a.heads + h;
+  const float* ml = a.ml + row * S * 2;
+  if (tid < 64) {
+    float mx = -INFINITY;
+    for (int s = tid; s < S; s += 64) mx = fmaxf(mx, ml[2 * s]);
+    mx = group_max<64>(mx);
+    float tot = 0.f;
+    for (int s = tid; s < S; s += 64) {
+      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f(ms - mx);
+      sw[s] = w;
+      tot += w * ml[2 * s + 1];
+    }
+    tot = group_sum<64>(tot);
+    if (tid == 0) stot = tot;
+  }
+  __syncthreads();
+  const int ln = tid % LN, way = tid / LN;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = way; s < S; s += WAYS) {
+    const f32x4 v = reinterpret_cast<const f32x4*>(a.part + (row * S + s) * HD)[ln];
+    const float w = sw[s];
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = fmaf(w, v[i], acc[i]);
+  }
+  sacc[tid] = acc;
+  __syncthreads();
+  if (tid < LN) {
+    for (int w = 1; w < WAYS; w++) {
+      const f32x4 v = sacc[w * LN + tid];
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[i] += v[i];
+    }
+    const float inv = stot == 0.f ? 0.f : 1.f / stot;
+    const long long at = (en.tok0 + blockIdx.y) * a.o_ts + h * a.o_hs + 4 * tid;
+#pragma unroll
+    for (int i = 0; i < 4; i++) kv4_store(a.out, at + i, round_storage_mode(acc[i] * inv, a.act16), a.q_dt);
+  }
+}
+
+// ---- page copies --------------------------------------------------------------------------------------------------------------------------------------
+struct CopyPagesArgs {
+  const unsigned char* src; unsigned char* dst;
+  long long src_pool, dst_pool, page;                         // bytes between the pools of two layers, and of a page (a multiple of 16)
+  long long src_pages, dst_pages;                             // pages of a pool
+  const int *from, *to; int n;                                // pairs; one outside of its pool is left out
+};
+// a workgroup a (16 KB piece of a page, pair, layer)
+constexpr int COPY_PIECE = 16384;
+static __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyPagesArgs a) {
+  const int pair = blockIdx.y;
+  const long long f = a.from[pair], t = a.to[pair];
+  if (f < 0 || f >= a.src_pages || t < 0 || t >= a.dst_pages) return;
+  const long long p0 = (long long)blockIdx.x * COPY_PIECE;
+  const u32x4* s = reinterpret_cast<const u32x4*>(a.src + blockIdx.z * a.src_pool + f * a.page + p0);
+  u32x4* d = reinterpret_cast<u32x4*>(a.dst + blockIdx.z * a.dst_pool + t * a.page + p0);
+  const long long left = (a.page - p0) / 16;
+  const int n = (int)(left < COPY_PIECE / 16 ? left : COPY_PIECE / 16);
+  u32x4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) { const int x = threadIdx.x + 256 * i; if (x < n) v[i] = load_nt(s + x); }
+#pragma unroll
+  for (int i = 0; i < 4; i++) { const int x = threadIdx.x + 256 * i; if (x < n) __builtin_nontemporal_store(v[i], d + x); }
+}
+
+}  // namespace tgx

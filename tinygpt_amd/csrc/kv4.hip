@@ -1,0 +1,239 @@
+// kv4.hip — the cache held in 4 bits: launches for a context's own use (kv4_* below, ctx.h) and the operators on device buffers of include/tgx.h
+// (kernels/kv4.h).  The operators know no context: device and stream come with the call, nothing is allocated, nothing waits.
+#include "ctx.h"
+#include "kernels/kv4.h"
+
+namespace {
+
+thread_local char g_op_err[256] = "";
+
+int op_err(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_op_err, sizeof g_op_err, fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+// the call's device is current inside, the caller's again afterwards
+struct OnDevice {
+  int before = -1, rc = TGX_OK;
+  explicit OnDevice(int device) {
+    int n = 0;
+    if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "no HIP device visible"); return; }
+    if (device < 0 || device >= n) { rc = op_err(TGX_ERR_INVALID, "device ordinal %d out of range [0,%d)", device, n); return; }
+    int cur = 0;
+    if (hipGetDevice(&cur) != hipSuccess) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "hipGetDevice failed"); return; }
+    if (cur == device) return;
+    if (hipSetDevice(device) != hipSuccess) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "hipSetDevice(%d) failed", device); return; }
+    before = cur;
+  }
+  ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+int num_cus_of(int device) {
+  static int cus[64];      // (every writer writes the same number)
+  if (device < 0 || device >= 64) return 256;
+  int n = __atomic_load_n(&cus[device], __ATOMIC_RELAXED);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) { (void)hipGetLastError(); return 256; }
+  __atomic_store_n(&cus[device], n, __ATOMIC_RELAXED);
+  return n;
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TGX_OK : op_err(TGX_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
+}
+
+int kv4_dt(int tgx) { return tgx == TGX_BF16 ? tgx::DT_BF16 : tgx == TGX_F16 ? tgx::DT_F16 : tgx == TGX_F32 ? tgx::DT_F32 : -1; }
+
+int check_cache(const tgx_kv4_cache* c, const tgx_kv4_batch* b, tgx::Kv4Args& a) {
+  if (!c || !b) return op_err(TGX_ERR_INVALID, "null argument");
+  if (c->head_dim != 64 && c->head_dim != 128) return op_err(TGX_ERR_UNSUPPORTED, "head_dim %d (64 and 128 are built)", c->head_dim);
+  if (c->kv_heads < 1 || c->kv_heads > 4096) return op_err(TGX_ERR_INVALID, "kv_heads %d out of range", c->kv_heads);
+  if (c->pages < 0 || c->pages > 0x7fffffff || c->seqs < 0 || c->table_len < 0 || c->table_stride < c->table_len || c->table_len > (0x7fffffff >> tgx::KV_BLOCK_SHIFT))
+    return op_err(TGX_ERR_INVALID, "cache: pages / seqs / table sizes out of range");
+  if (b->entries < 0 || b->entries > 65535 || b->tokens < 0 || b->tokens > 0x7fffffff || b->max_count < 0) return op_err(TGX_ERR_INVALID, "batch: entries / tokens / max_count out of range");
+  if (!b->offsets && b->tokens != b->entries) return op_err(TGX_ERR_INVALID, "batch: %lld tokens of %d entries without offsets", (long long)b->tokens, b->entries);
+  if (b->entries && (!c->pool || !c->table || !b->start)) return op_err(TGX_ERR_INVALID, "null argument");
+  if ((uintptr_t)c->pool & 15) return op_err(TGX_ERR_INVALID, "the pool is not aligned to 16 bytes");
+  a.pool = (unsigned int*)c->pool; a.pages = c->pages; a.table = c->table; a.table_stride = c->table_stride; a.table_len = c->table_len; a.seqs = c->seqs;
+  a.kv_heads = c->kv_heads;
+  a.entries = b->entries; a.max_count = b->offsets ? (int)std::min<int64_t>(b->max_count, b->tokens) : std::min(b->max_count, 1); a.tokens = b->tokens;
+  a.seq = b->seq; a.start = b->start; a.offsets = b->offsets;
+  return TGX_OK;
+}
+
+int check_rows(const tgx_kv4_rows* r, const char* name) {
+  if (!r || !r->data) return op_err(TGX_ERR_INVALID, "%s: null argument", name);
+  if (kv4_dt(r->dtype) < 0) return op_err(TGX_ERR_INVALID, "%s: unknown dtype %d", name, r->dtype);
+  if ((uintptr_t)r->data % (r->dtype == TGX_F32 ? 4 : 2)) return op_err(TGX_ERR_INVALID, "%s: not aligned to its elements", name);
+  return TGX_OK;
+}
+
+int check_kv(const tgx_kv4_rows* k, const tgx_kv4_rows* v, tgx::Kv4Args& a) {
+  int rc;
+  if ((rc = check_rows(k, "k")) || (rc = check_rows(v, "v"))) return rc;
+  if (k->dtype != v->dtype) return op_err(TGX_ERR_INVALID, "k and v have different dtypes");
+  a.k = k->data; a.v = v->data; a.kv_dt = kv4_dt(k->dtype); a.k_ts = k->token_stride; a.k_hs = k->head_stride; a.v_ts = v->token_stride; a.v_hs = v->head_stride;
+  return TGX_OK;
+}
+
+// blocks of 32 positions that an entry of n tokens may touch
+int blocks_of(int n) { return (n + 30) / 32 + 1; }
+
+}  // namespace
+
+void kv4_launch_append(const tgx::Kv4Args& a, int hd, hipStream_t s) {
+  if (!a.entries || !a.max_count) return;
+  if (a.max_count == 1) {
+    const dim3 grid(a.kv_heads, a.entries);
+    if (hd == 64) hipLaunchKernelGGL(tgx::kv4_append_token_kernel<64>, grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL(tgx::kv4_append_token_kernel<128>, grid, dim3(64), 0, s, a);
+    return;
+  }
+  const dim3 grid(a.kv_heads, blocks_of(a.max_count), a.entries);
+  TGX_DT_SWITCH(a.kv_dt,
+    if (hd == 64) hipLaunchKernelGGL((tgx::kv4_append_block_kernel<64, DT>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_append_block_kernel<128, DT>), grid, dim3(64), 0, s, a);)
+}
+
+void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s) {
+  if (!a.entries || !a.max_count) return;
+  const dim3 grid(a.kv_heads, blocks_of(a.max_count), a.entries);
+  TGX_DT_SWITCH(a.kv_dt,
+    if (hd == 64) hipLaunchKernelGGL((tgx::kv4_read_kernel<64, DT>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_read_kernel<128, DT>), grid, dim3(64), 0, s, a);)
+}
+
+template <int HD, int TERMS>
+static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
+  const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries), blk(256);
+  if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 1, 4, TERMS>), grid, blk, 0, s, a);
+  else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 2, 4, TERMS>), grid, blk, 0, s, a);
+  else hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 2, 1, TERMS>), grid, blk, 0, s, a);
+}
+
+// a.splits, a.part, a.ml follow from the plan and the workspace here; with keys and values to append that the attention launch does not append itself, an append launch first
+void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws, hipStream_t s) {
+  if (!a.entries || !a.max_count) return;
+  if (a.k && a.max_count > 1) { kv4_launch_append(a, hd, s); a.k = a.v = nullptr; }
+  const size_t rows = (size_t)a.tokens * a.heads;
+  a.splits = p.splits;
+  a.part = ws; a.ml = ws + rows * p.splits * hd;
+  const bool two = a.q_dt != tgx::DT_BF16;
+  if (hd == 64) { if (two) launch_attend<64, 2>(a, p, s); else launch_attend<64, 1>(a, p, s); }
+  else { if (two) launch_attend<128, 2>(a, p, s); else launch_attend<128, 1>(a, p, s); }
+  if (p.splits > 1) {
+    const dim3 grid(a.heads, a.max_count, a.entries);
+    if (hd == 64) hipLaunchKernelGGL(tgx::kv4_combine_kernel<64>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(tgx::kv4_combine_kernel<128>, grid, dim3(256), 0, s, a);
+  }
+}
+
+void launch_copy_pages(const tgx::CopyPagesArgs& a, int layers, hipStream_t s) {
+  if (!a.n || !layers || !a.page) return;
+  hipLaunchKernelGGL(tgx::copy_pages_kernel, dim3((unsigned)((a.page + tgx::COPY_PIECE - 1) / tgx::COPY_PIECE), a.n, layers), dim3(256), 0, s, a);
+}
+
+extern "C" {
+
+const char* tgx_op_last_error(void) { return g_op_err; }
+
+int64_t tgx_kv4_page_bytes(int kv_heads, int head_dim) {
+  if ((head_dim != 64 && head_dim != 128) || kv_heads < 1 || kv_heads > 4096) return -1;
+  return (int64_t)tgx::kv4_page_words(kv_heads, head_dim) * 4;
+}
+
+int tgx_kv4_append(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream) {
+  tgx::Kv4Args a{};
+  int rc;
+  if ((rc = check_cache(cache, batch, a))) return rc;
+  if (!a.entries) return TGX_OK;
+  if ((rc = check_kv(k, v, a))) return rc;
+  if (blocks_of(a.max_count) > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
+  if (!a.max_count || !a.tokens) return TGX_OK;
+  OnDevice on(device);
+  if (on.rc) return on.rc;
+  kv4_launch_append(a, cache->head_dim, (hipStream_t)stream);
+  return launched("kv4 append");
+}
+
+int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream) {
+  tgx::Kv4Args a{};
+  int rc;
+  if ((rc = check_cache(cache, batch, a))) return rc;
+  if (!a.entries) return TGX_OK;
+  if ((rc = check_kv(k, v, a))) return rc;
+  if (blocks_of(a.max_count) > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
+  if (!a.max_count || !a.tokens) return TGX_OK;
+  OnDevice on(device);
+  if (on.rc) return on.rc;
+  kv4_launch_read(a, cache->head_dim, (hipStream_t)stream);
+  return launched("kv4 read");
+}
+
+static int attend_args(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, int heads, int window, int64_t max_keys, tgx::Kv4Args& a) {
+  int rc;
+  if ((rc = check_cache(cache, batch, a))) return rc;
+  if (heads < 1 || heads % cache->kv_heads) return op_err(TGX_ERR_INVALID, "%d query heads over %d key / value heads", heads, cache->kv_heads);
+  if (heads / cache->kv_heads > 16) return op_err(TGX_ERR_UNSUPPORTED, "GQA group size %d > 16", heads / cache->kv_heads);
+  if (heads > 65535) return op_err(TGX_ERR_UNSUPPORTED, "%d query heads", heads);
+  if (window < 0 || window > (1 << 30)) return op_err(TGX_ERR_INVALID, "window %d out of range", window);
+  if (max_keys < 0 || max_keys > 0x7fffffff) return op_err(TGX_ERR_INVALID, "max_keys out of range");
+  if (a.max_count > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d > 65535", a.max_count);
+  a.heads = heads; a.group = heads / cache->kv_heads; a.window = window;
+  return TGX_OK;
+}
+
+int64_t tgx_kv4_attend_workspace(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, int heads, int window, int64_t max_keys, int device) {
+  tgx::Kv4Args a{};
+  if (attend_args(cache, batch, heads, window, max_keys, a)) return -1;
+  if (!a.entries || !a.max_count || !a.tokens) return 0;
+  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, window, max_keys, num_cus_of(device));
+  return (int64_t)tgx::kv4_part_floats(p, a.tokens * heads, cache->head_dim) * 4;
+}
+
+int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* q, int heads, const tgx_kv4_rows* k, const tgx_kv4_rows* v, float scale, int window,
+                   int64_t max_keys, const tgx_kv4_rows* out, void* workspace, int64_t workspace_bytes, int device, void* stream) {
+  tgx::Kv4Args a{};
+  int rc;
+  if ((rc = attend_args(cache, batch, heads, window, max_keys, a))) return rc;
+  if (!a.entries) return TGX_OK;
+  if ((rc = check_rows(q, "q")) || (rc = check_rows(out, "out"))) return rc;
+  if (q->dtype != out->dtype) return op_err(TGX_ERR_INVALID, "q and out have different dtypes");
+  if (!k != !v) return op_err(TGX_ERR_INVALID, "k and v come together");
+  if (k && (rc = check_kv(k, v, a))) return rc;
+  if (!std::isfinite(scale)) return op_err(TGX_ERR_INVALID, "scale is not finite");
+  a.q = q->data; a.out = out->data; a.q_dt = kv4_dt(q->dtype); a.q_ts = q->token_stride; a.q_hs = q->head_stride; a.o_ts = out->token_stride; a.o_hs = out->head_stride;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  if (!a.max_count || !a.tokens) return TGX_OK;
+  OnDevice on(device);
+  if (on.rc) return on.rc;
+  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, window, max_keys, num_cus_of(device));
+  const int64_t need = (int64_t)tgx::kv4_part_floats(p, a.tokens * heads, cache->head_dim) * 4;
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return op_err(TGX_ERR_INVALID, "workspace: %lld bytes aligned to 16 are needed", (long long)need);
+  if (p.tiles > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
+  kv4_launch_attend(a, p, cache->head_dim, (float*)workspace, (hipStream_t)stream);
+  return launched("kv4 attention");
+}
+
+int tgx_copy_pages(const void* src, int64_t src_pages, int64_t src_stride, void* dst, int64_t dst_pages, int64_t dst_stride, int layers, int64_t page_bytes, const int32_t* from,
+                   const int32_t* to, int n, int device, void* stream) {
+  if (n < 0 || n > 65535 || layers < 0 || layers > 65535) return op_err(TGX_ERR_INVALID, "%d pairs, %d layers (0 .. 65535)", n, layers);
+  if (src_pages < 0 || dst_pages < 0 || page_bytes < 0 || src_stride < 0 || dst_stride < 0) return op_err(TGX_ERR_INVALID, "sizes out of range");
+  if (!n || !layers || !page_bytes) return TGX_OK;
+  if (!src || !dst || !from || !to) return op_err(TGX_ERR_INVALID, "null argument");
+  if (page_bytes % 16 || src_stride % 16 || dst_stride % 16 || ((uintptr_t)src & 15) || ((uintptr_t)dst & 15)) return op_err(TGX_ERR_INVALID, "pools, strides and pages are multiples of 16 bytes");
+  if ((page_bytes + tgx::COPY_PIECE - 1) / tgx::COPY_PIECE > 0x7fffffff) return op_err(TGX_ERR_INVALID, "sizes out of range");
+  OnDevice on(device);
+  if (on.rc) return on.rc;
+  tgx::CopyPagesArgs a{};
+  a.src = (const unsigned char*)src; a.dst = (unsigned char*)dst; a.src_pool = src_stride; a.dst_pool = dst_stride; a.page = page_bytes; a.src_pages = src_pages; a.dst_pages = dst_pages;
+  a.from = from; a.to = to; a.n = n;
+  launch_copy_pages(a, layers, (hipStream_t)stream);
+  return launched("page copy");
+}
+
+}  // extern "C"

@@ -1,0 +1,93 @@
+// kv4_plan.h — the cache held in 4 bits (kernels/kv4.h): its arguments, where a code lies, what a call's entry brings, which pages it reads and how its attention is
+// divided, as plain arithmetic (no HIP call: tests go through it on the CPU, the kernels through the same functions).
+#pragma once
+#include <algorithm>
+#include <cstddef>
+
+#if defined(__HIPCC__)
+#define TGX_KV4 __host__ __device__ __forceinline__
+#else
+#define TGX_KV4 inline
+#endif
+
+namespace tgx {
+
+constexpr int KV4_PAGE = 128, KV4_PAGE_SHIFT = 7, KV4_BLK = 32;      // tokens of a page, of a block
+
+struct Kv4Args {
+  unsigned int* pool; long long pages;                        // pages of one layer
+  const int* table; int table_stride, table_len, seqs;        // [seqs][table_stride], table_len entries of a row count; a page outside [0, pages) counts as one without tokens
+  int kv_heads;
+  int entries, max_count; long long tokens;                   // the batch: entries of consecutive tokens of a sequence each
+  const int *seq, *start, *offsets;                           // seq: entry's table row (null: entry e is row e); start: position of its first token; offsets [entries + 1] into the tokens (null: one token each)
+  // keys and values that join (append), or that come out (read): element (token, kv head, channel) at token * k_ts + head * k_hs + (position % KV4_PAGE) * slot_s + channel
+  void *k, *v; int kv_dt; long long k_ts, k_hs, v_ts, v_hs, slot_s;
+  // attention
+  const void* q; void* out; int q_dt; long long q_ts, q_hs, o_ts, o_hs;
+  int heads, group; float scale_log2;                         // score scale * log2(e)
+  int window;                                                 // > 0: position p sees keys p - window + 1 .. p
+  int splits; float *part, *ml;                               // splits > 1: [token * heads + head][splits][HD] sums, [..][splits][2] (maximum, denominator)
+  int act16;                                                  // outputs rounded to the storage type: 0 no, 1 bf16, 2 fp16 (option act.round16 of a model)
+};
+
+// tokens, first token and position of entry e; count 0 where the entry names no sequence or its tokens are not all in the batch
+struct Kv4Entry { int seq, start, count; long long tok0; };
+TGX_KV4 Kv4Entry kv4_entry(const Kv4Args& a, int e) {
+  Kv4Entry n;
+  n.seq = a.seq ? a.seq[e] : e;
+  n.start = a.start[e] < -(1 << 30) ? -(1 << 30) : a.start[e];
+  const long long o0 = a.offsets ? a.offsets[e] : e, c = a.offsets ? a.offsets[e + 1] - o0 : 1;
+  n.tok0 = o0;
+  n.count = (int)(c < a.max_count ? c : a.max_count);
+  if (o0 < 0 || c < 0 || o0 + n.count > a.tokens || n.seq < 0 || n.seq >= a.seqs || n.start > 0x7fffffff - n.count) n.count = 0;
+  return n;
+}
+
+// the words of a page's head, or null where the table names no page
+TGX_KV4 unsigned int* kv4_page(const Kv4Args& a, int seq, int b, int kvh, int hd) {
+  if (b < 0 || b >= a.table_len) return nullptr;
+  const int p = a.table[(long long)seq * a.table_stride + b];
+  if (p < 0 || p >= a.pages) return nullptr;
+  return a.pool + ((size_t)p * a.kv_heads + kvh) * (size_t)(36 * hd);
+}
+TGX_KV4 size_t kv4_page_words(int kv_heads, int hd) { return (size_t)kv_heads * 36 * hd; }
+
+// places in a block's 9 HD words: of the word that holds a key code (token t of the block, channel), a value code, a group's parameters; and a code's first bit
+TGX_KV4 int kv4_word(int i, int q, int r) { return ((i >> 2) * 64 + 16 * q + r) * 4 + (i & 3); }
+TGX_KV4 int kv4_key_word(int hd, int t, int ch) { return kv4_word((t >> 4) * (hd / 32) + (ch >> 5), (ch >> 3) & 3, t & 15); }
+TGX_KV4 int kv4_value_word(int hd, int t, int ch) { return 4 * hd + kv4_word(ch >> 4, (t & 15) >> 2, ch & 15); }
+TGX_KV4 int kv4_param_word(int hd, int t, int value, int group) { return 8 * hd + (t * 2 + value) * (hd / 64) + group; }
+TGX_KV4 int kv4_code_bit(int e) { return 4 * ((e >> 1) + 4 * (e & 1)); }
+TGX_KV4 int kv4_key_bit(int ch) { return kv4_code_bit(ch & 7); }
+TGX_KV4 int kv4_value_bit(int t) { return kv4_code_bit((t & 3) + 4 * ((t >> 4) & 1)); }
+TGX_KV4 int kv4_value_token(int q, int e) { return e < 4 ? 4 * q + e : 12 + 4 * q + e; }      // the token of a value word's code e
+
+// pages [lo, hi) that split `split` of `splits` walks for columns at positions first .. last
+struct Kv4Range { int lo, hi; };
+TGX_KV4 Kv4Range kv4_range(int first, int last, int window, int table_len, int split, int splits) {
+  const int key_lo = window > 0 && first - window + 1 > 0 ? first - window + 1 : 0;
+  const int lo = key_lo >> KV4_PAGE_SHIFT, all = last < 0 ? 0 : (last >> KV4_PAGE_SHIFT) + 1, hi = all < table_len ? all : table_len;
+  const int per = hi > lo ? (hi - lo + splits - 1) / splits : 0;
+  const long long p0 = lo + (long long)split * per, p1 = p0 + per;
+  return Kv4Range{(int)(p0 < hi ? p0 : hi), (int)(p1 < hi ? p1 : hi)};
+}
+
+// How a batch's attention is divided: kw 4 = the waves of a workgroup share nt * 16 columns (token, query head) and divide the keys, kw 1 = they divide the columns;
+// tiles workgroups of columns, splits of the keys between workgroups
+struct Kv4Plan { int kw, nt, tiles, splits; };
+inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int window, long long max_keys, int num_cus) {
+  Kv4Plan p;
+  const long long cols = (long long)max_count * group;
+  p.kw = cols <= 32 ? 4 : 1;
+  p.nt = p.kw == 4 ? (cols <= 16 ? 1 : 2) : 2;
+  const int per = 16 * p.nt * (p.kw == 4 ? 1 : 4);
+  p.tiles = (int)((cols + per - 1) / per);
+  const long long keys = window > 0 ? std::min<long long>(max_keys, (long long)window + max_count) : max_keys;
+  const long long pages = std::max<long long>(1, (keys + KV4_PAGE - 1) / KV4_PAGE);
+  const long long wgs = std::max<long long>(1, (long long)entries * kv_heads * p.tiles);
+  p.splits = (int)std::max<long long>(1, std::min<long long>({(4ll * num_cus + wgs - 1) / wgs, pages, 256}));
+  return p;
+}
+inline size_t kv4_part_floats(const Kv4Plan& p, long long rows, int hd) { return p.splits > 1 ? (size_t)rows * p.splits * (hd + 2) : 0; }      // workspace of the splits' records
+
+}  // namespace tgx

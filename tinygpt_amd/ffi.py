@@ -50,6 +50,22 @@ class TgxError(RuntimeError):
         self.status = status
 
 
+class Kv4CacheArg(ctypes.Structure):
+    """struct tgx_kv4_cache (include/tgx.h): the pages of one layer of a 4-bit cache and the page table, on the device"""
+    _fields_ = [("pool", c_void_p), ("pages", c_int64), ("table", c_void_p), ("table_stride", c_int32), ("table_len", c_int32), ("seqs", c_int32),
+                ("kv_heads", c_int32), ("head_dim", c_int32)]
+
+
+class Kv4BatchArg(ctypes.Structure):
+    """struct tgx_kv4_batch: a call's tokens in entries of consecutive positions"""
+    _fields_ = [("entries", c_int32), ("max_count", c_int32), ("tokens", c_int64), ("seq", c_void_p), ("start", c_void_p), ("offsets", c_void_p)]
+
+
+class Kv4RowsArg(ctypes.Structure):
+    """struct tgx_kv4_rows: [tokens][heads][head_dim] on the device"""
+    _fields_ = [("data", c_void_p), ("dtype", c_int32), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/tgx.h declares
 ABI = {
     "device_count": (c_int, [POINTER(c_int)]),
@@ -84,6 +100,14 @@ ABI = {
     "set_logits": (c_int, [c_void_p, POINTER(c_float), c_int]),
     "bytes_per_token": (c_int64, [c_void_p, c_int64]),
     "abi_version": (c_int, []),
+    "kv4_page_bytes": (c_int64, [c_int, c_int]),
+    "kv4_append": (c_int, [POINTER(Kv4CacheArg), POINTER(Kv4BatchArg), POINTER(Kv4RowsArg), POINTER(Kv4RowsArg), c_int, c_void_p]),
+    "kv4_read": (c_int, [POINTER(Kv4CacheArg), POINTER(Kv4BatchArg), POINTER(Kv4RowsArg), POINTER(Kv4RowsArg), c_int, c_void_p]),
+    "kv4_attend_workspace": (c_int64, [POINTER(Kv4CacheArg), POINTER(Kv4BatchArg), c_int, c_int, c_int64, c_int]),
+    "kv4_attend": (c_int, [POINTER(Kv4CacheArg), POINTER(Kv4BatchArg), POINTER(Kv4RowsArg), c_int, POINTER(Kv4RowsArg), POINTER(Kv4RowsArg), c_float, c_int, c_int64,
+                           POINTER(Kv4RowsArg), c_void_p, c_int64, c_int, c_void_p]),
+    "copy_pages": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "op_last_error": (c_char_p, []),
 }
 
 
