@@ -268,16 +268,16 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
 // ---- attention ------------------------------------------------------------------------------------------------------------------------------------------
 // S^T = K Q^T with the codes as the operand: a score is sum_g step_g (q_g . (128 + n_g)) + (lo_g - 128 step_g) sum(q_g), so that a product of 16 tokens x 16 query
 // columns (column = token of the entry, query head of the kv head) costs two fused multiply-adds a score and group and no value is unpacked.  O = P V the same
-// way: the weights p step_g (bf16, TERMS of them) meet 128 + n; what the 128 adds is taken off with the weights' own sum (a product with ones: the same rounded
+// way: the weights p step_g (bf16, TP terms of them) meet 128 + n; what the 128 adds is taken off with the weights' own sum (a product with ones: the same rounded
 // weights), the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A operand
 // of P V, whose contraction runs over the tokens in the order of the value words.
-// TERMS: 16-bit terms of a query and of a weight.  Two keep what 32-bit inputs bring (2^-17); queries in bf16 are one term exactly.
-// KW = 4: the waves of a workgroup divide the keys (wave w: block w of every page), all columns in each; their sums meet in LDS.  KW = 1: they divide the
-// columns and walk the same keys.
-__device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
+// TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17) leave an output
+// in 16 bits what its own rounding leaves, three one in 32.  One term (2^-9, as coarse as an output in bf16) is taken off the levels' middle: 136 in the place of 128
+// and lo + 8 step in the place of lo, so that its rounding meets numbers as large as the values and not as their spread.
+__device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w, unsigned int mask, unsigned int off) {
   u32x4 f;
 #pragma unroll
-  for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & mask) | off;
   return __builtin_bit_cast(bf16x8_t, f);
 }
 __device__ __forceinline__ float kv4_max_quarters(float v) {      // over the lanes of equal r
@@ -288,267 +288,418 @@ __device__ __forceinline__ float kv4_sum_quarters(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
+// eight neighbouring channels of a row of a runtime type
+__device__ __forceinline__ void kv4_load8(const void* p, long long i, int dt, float x[8]) {
+  if (dt == DT_F32) {
+    const float* f = static_cast<const float*>(p) + i;
+    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) slice_unpack<DT_F32>(load_slice<DT_F32>(f, 0), x);
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = f[e];
+    }
+    return;
+  }
+  const unsigned short* u = static_cast<const unsigned short*>(p) + i;
+  u32x4 w;
+  if ((reinterpret_cast<uintptr_t>(u) & 15) == 0) w = *reinterpret_cast<const u32x4*>(u);
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = u[2 * e] | ((unsigned int)u[2 * e + 1] << 16);
+  }
+  Slice8<DT_BF16> s{w};
+  if (dt == DT_BF16) slice_unpack<DT_BF16>(s, x);
+  else slice_unpack<DT_F16>(Slice8<DT_F16>{w}, x);
+}
+__device__ __forceinline__ void kv4_store4(void* p, long long i, const f32x4 v, int dt) {
+  if (dt == DT_F32) {
+    float* f = static_cast<float*>(p) + i;
+    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) *reinterpret_cast<f32x4*>(f) = v;
+    else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[e] = v[e];
+    }
+    return;
+  }
+  unsigned short* u = static_cast<unsigned short*>(p) + i;
+  unsigned short h[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) h[e] = dt == DT_BF16 ? f32_to_bf16(v[e]) : f32_to_f16_bits(v[e]);
+  if ((reinterpret_cast<uintptr_t>(u) & 7) == 0) *reinterpret_cast<u32x2*>(u) = u32x2{h[0] | ((unsigned int)h[1] << 16), h[2] | ((unsigned int)h[3] << 16)};
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) u[e] = h[e];
+  }
+}
 
-template <int HD, int NT, int KW, int TERMS>
-__global__ __launch_bounds__(256) void kv4_attend_kernel(const Kv4Args a) {
-  constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64;
+// a block's codes and parameters on their way: key and value words as operands, the parameters of token (lane & 31)
+template <int HD> struct Kv4Raw {
+  u32x4 k[HD / 64], v[HD / 64];
+  unsigned int p[HD / 32];
+  __device__ __forceinline__ void load(const unsigned int* blk, int lane) {
+#pragma unroll
+    for (int i = 0; i < HD / 64; i++) k[i] = load_nt(reinterpret_cast<const u32x4*>(blk) + i * 64 + lane);
+    if constexpr (HD == 128) { const u32x4 w = load_nt(reinterpret_cast<const u32x4*>(blk + 8 * HD) + (lane & 31)); p[0] = w[0]; p[1] = w[1]; p[2] = w[2]; p[3] = w[3]; }
+    else { const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(blk + 8 * HD) + (lane & 31)); p[0] = w[0]; p[1] = w[1]; }
+#pragma unroll
+    for (int i = 0; i < HD / 64; i++) v[i] = load_nt(reinterpret_cast<const u32x4*>(blk + 4 * HD) + i * 64 + lane);
+  }
+};
+
+// The sums of NT tiles of 16 query columns over the blocks that a wave walks.
+template <int HD, int NT, int TQ, int TP>
+struct Kv4Sums {
+  static constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16;
+  static constexpr bool CENTRE = TP == 1;
+  bf16x8_t qf[NT][CH][TQ];
+  float qsum[NT][G];
+  int pos[NT];                                                // a column's position; -1: no column
+  f32x4 o[NT][CT], ones[NT][G];
+  float m[NT], l[NT], lov[NT][G];                             // m: the reference of the weights, in scores before the scale
+
+  __device__ __forceinline__ void start(const Kv4Args& a, const Kv4Entry& en, int kvh, int col0, int ncol, int q4, int r16) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int c = col0 + 16 * t + r16, cc = min(c, ncol - 1), i = en.count == 1 ? 0 : cc / a.group, h = kvh * a.group + cc - i * a.group;
+      pos[t] = c < ncol ? en.start + i : -1;
+      const long long base = (en.tok0 + i) * a.q_ts + h * a.q_hs + 8 * q4;
+      m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; g++) { qsum[t][g] = 0.f; lov[t][g] = 0.f; ones[t][g] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+#pragma unroll
+      for (int x = 0; x < CT; x++) o[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ch = 0; ch < CH; ch++) {
+        float x[8];
+        kv4_load8(a.q, base + 32 * ch, a.q_dt, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
+#pragma unroll
+        for (int term = 0; term < TQ; term++) {
+          u32x4 f;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            f[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+            qsum[t][ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
+            x[2 * e] -= bf16_lo(f[e]); x[2 * e + 1] -= bf16_hi(f[e]);
+          }
+          qf[t][ch][term] = __builtin_bit_cast(bf16x8_t, f);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; g++) qsum[t][g] = kv4_sum_quarters(qsum[t][g]);
+    }
+  }
+
+  // one block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters (which every lane needs of the four tokens of its scores).  MASK: some column does not see
+  // some token of the block; what is not seen is selected away, whatever it holds.
+  template <bool MASK>
+  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+    const int q4 = lane >> 4;
+    constexpr int PW = HD / 32;                               // parameter words of a token: keys, then values
+    if constexpr (PW == 4) *reinterpret_cast<u32x4*>(sp + (lane & 31) * 4) = u32x4{raw.p[0], raw.p[1], raw.p[2], raw.p[3]};
+    else *reinterpret_cast<u32x2*>(sp + (lane & 31) * 2) = u32x2{raw.p[0], raw.p[1]};
+    wave_fence();
+    unsigned int par[2][4][PW];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int w = 0; w < PW; w++) par[i][r][w] = sp[(16 * i + 4 * q4 + r) * PW + w];
+    wave_fence();
+    f32x4 sc[NT][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        bf16x8_t kf[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(raw.k[x >> 2][x & 3], mask, off); }
+        float st[4], z[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) { st[r] = bf16_hi(par[i][r][g]); z[r] = fmaf(-128.f, st[r], bf16_lo(par[i][r][g])); }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int term = 0; term < TQ; term++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], qf[t][2 * g + c][term], d, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; r++) sc[t][i][r] = fmaf(st[r], d[r], g == 0 ? z[r] * qsum[t][g] : fmaf(z[r], qsum[t][g], sc[t][i][r]));
+        }
+      }
+    }
+    u32x4 pf[NT][G][TP];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      bool seen[2][4];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int j = t0 + 16 * i + 4 * q4 + r;
+          seen[i][r] = !MASK || (j <= pos[t] && (window <= 0 || j > pos[t] - window));
+          if (MASK && !seen[i][r]) sc[t][i][r] = -INFINITY;
+          mx = fmaxf(mx, sc[t][i][r]);
+        }
+      mx = kv4_max_quarters(mx);
+      // the sums keep their reference until a maximum passes it by 8 in the exponent (weights up to 256 then): few blocks rescale
+      if (__any(mx > m[t] + gap)) {
+        const float nm = fmaxf(m[t], mx), f = nm > m[t] ? __builtin_amdgcn_exp2f((m[t] - nm) * scale) : 1.f;
+        m[t] = nm;
+        l[t] *= f;
+#pragma unroll
+        for (int g = 0; g < G; g++) lov[t][g] *= f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float fr = __shfl(f, 4 * q4 + r, 64);
+#pragma unroll
+          for (int c = 0; c < CT; c++) o[t][c][r] *= fr;
+#pragma unroll
+          for (int g = 0; g < G; g++) ones[t][g][r] *= fr;
+        }
+      }
+      const float ref = -m[t] * scale;
+      float p[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          p[i][r] = __builtin_amdgcn_exp2f(fmaf(sc[t][i][r], scale, ref));
+          if (MASK && !seen[i][r]) p[i][r] = 0.f;
+          l[t] += p[i][r];
+        }
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        float ps[8];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const unsigned int w = par[i][r][G + g];
+            const float st = bf16_hi(w), lo = CENTRE ? fmaf(8.f, st, bf16_lo(w)) : bf16_lo(w);
+            ps[4 * i + r] = MASK && !seen[i][r] ? 0.f : p[i][r] * st;
+            lov[t][g] = MASK && !seen[i][r] ? lov[t][g] : fmaf(p[i][r], lo, lov[t][g]);
+          }
+#pragma unroll
+        for (int term = 0; term < TP; term++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            pf[t][g][term][e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
+            if (term + 1 < TP) { ps[2 * e] -= bf16_lo(pf[t][g][term][e]); ps[2 * e + 1] -= bf16_hi(pf[t][g][term][e]); }
+          }
+      }
+    }
+    const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int term = 0; term < TP; term++) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][g][term]), one8, ones[t][g], 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int x = 4 * g + c;
+        const bf16x8_t vf = kv4_frag(raw.v[x >> 2][x & 3], mask, off);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int term = 0; term < TP; term++) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][g][term]), vf, o[t][x], 0, 0, 0);
+      }
+    }
+  }
+
+  // o becomes the columns' sums, l their denominators (over the four quarters)
+  __device__ __forceinline__ void finish(int q4) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      l[t] = kv4_sum_quarters(l[t]);
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const float lg = kv4_sum_quarters(lov[t][g]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float add = fmaf(CENTRE ? -136.f : -128.f, ones[t][g][r], __shfl(lg, 4 * q4 + r, 64));
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
+        }
+      }
+    }
+  }
+};
+
+// Few columns (a token's query heads, or a few tokens'): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
+// The next block is on its way while one is worked on.  The waves' sums meet once in LDS, where a thread takes four channels of a column through all waves.
+template <int HD, int NT, int KW, int TQ, int TP>
+__global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args a) {
+  typedef Kv4Sums<HD, NT, TQ, TP> Sums;
+  constexpr int CT = Sums::CT;
+  extern __shared__ __attribute__((aligned(16))) float kv4_lds[];
+  __shared__ __attribute__((aligned(16))) unsigned int s_par[KW][HD];
+  __shared__ float s_ml[KW][16][2];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
-  const int ncol = en.count * a.group;
-  const int col0 = (KW == 4 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wv) * 16 * NT;
-  if (col0 >= ncol) return;      // (KW 1 has no barrier)
-  // this token's key and value first, by the workgroup whose pages hold its place (single tokens)
-  int my_pos[NT];
-  bool valid[NT];
-  const int first = en.start + min(col0, ncol - 1) / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;      // positions of the columns
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int c = col0 + 16 * t + r16;
-    valid[t] = c < ncol;
-    my_pos[t] = valid[t] ? en.start + c / a.group : -1;
-  }
-  // queries: column r, channels 32 c + 8 q .. + 7
-  bf16x8_t qf[NT][CH][TERMS];
-  float qsum[NT][G];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int c = min(col0 + 16 * t + r16, ncol - 1), i = c / a.group, h = kvh * a.group + c % a.group;
-    const long long base = (en.tok0 + i) * a.q_ts + h * a.q_hs + 8 * q4;
-#pragma unroll
-    for (int g = 0; g < G; g++) qsum[t][g] = 0.f;
-#pragma unroll
-    for (int ch = 0; ch < CH; ch++) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = kv4_load(a.q, base + 32 * ch + e, a.q_dt);
-      bf16_t hi[8], lo[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        split16<DT_BF16>(x[e], hi[e], lo[e]);
-        qsum[t][ch / 2] += TERMS == 2 ? bf16_to_f32(hi[e]) + bf16_to_f32(lo[e]) : bf16_to_f32(hi[e]);
-      }
-      u32x4 f, fl;
-#pragma unroll
-      for (int e = 0; e < 4; e++) { f[e] = hi[2 * e] | ((unsigned)hi[2 * e + 1] << 16); fl[e] = lo[2 * e] | ((unsigned)lo[2 * e + 1] << 16); }
-      qf[t][ch][0] = __builtin_bit_cast(bf16x8_t, f);
-      if constexpr (TERMS == 2) qf[t][ch][1] = __builtin_bit_cast(bf16x8_t, fl);
-    }
-#pragma unroll
-    for (int g = 0; g < G; g++) qsum[t][g] = kv4_sum_quarters(qsum[t][g]);
-  }
-  f32x4 o[NT][CT], ones[NT][G];
-  float m[NT], l[NT], lov[NT][G];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    m[t] = -INFINITY; l[t] = 0.f;
-#pragma unroll
-    for (int g = 0; g < G; g++) { lov[t][g] = 0.f; ones[t][g] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-#pragma unroll
-    for (int c = 0; c < CT; c++) o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  const int key_hi = last + 1, key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;      // keys that some column sees
+  const int ncol = en.count * a.group, col0 = (int)blockIdx.y * 16 * NT;
+  if (col0 >= ncol) return;
+  const int first = en.start + (en.count == 1 ? 0 : col0 / a.group), last = en.start + (en.count == 1 ? 0 : min(col0 + 16 * NT - 1, ncol - 1) / a.group);      // positions of the columns
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
-  const int pg0 = rg.lo, pg1 = rg.hi;
-  if (KW == 4 && NT == 1 && a.k != nullptr && en.count == 1 && en.start >= 0) {
-    const int b = en.start >> KV_BLOCK_SHIFT;
-    if (b >= pg0 && b < pg1) {
+  // this token's key and value first, by the workgroup whose pages hold its place (single tokens)
+  if (NT == 1 && a.k != nullptr && en.count == 1 && en.start >= 0) {
+    const int b = en.start >> KV4_PAGE_SHIFT;
+    if (b >= rg.lo && b < rg.hi) {
       unsigned int* page = kv4_page(a, en.seq, b, kvh, HD);
       if (page && wv == 0) kv4_append_one<HD, true>(a, page, en.tok0, en.start, kvh);
       __syncthreads();
     }
   }
-  for (int pg = pg0; pg < pg1; pg++) {
-    const unsigned int* page = kv4_page(a, en.seq, pg, kvh, HD);
-    if (!page) continue;
-#pragma unroll 1
-    for (int b = KW == 4 ? wv : 0; b < (KW == 4 ? wv + 1 : 4); b++) {
-      const int t0 = pg * KV_BLOCK + b * KV4_BLK;
-      if (t0 >= key_hi || t0 + KV4_BLK <= key_lo) continue;
-      const unsigned int* blk = page + (size_t)b * kv4_block_words<HD>();
-      u32x4 kw[PARTS], vw[PARTS], pw[2][2 * G];
-#pragma unroll
-      for (int p = 0; p < PARTS; p++) kw[p] = reinterpret_cast<const u32x4*>(blk)[p * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2 * G; j++) pw[i][j] = reinterpret_cast<const u32x4*>(blk + 8 * HD + (16 * i + 4 * q4) * 2 * G)[j];
-#pragma unroll
-      for (int p = 0; p < PARTS; p++) vw[p] = reinterpret_cast<const u32x4*>(blk + 4 * HD)[p * 64 + lane];
-      auto par = [&](int i, int r, int kv, int g) -> unsigned int { const int x = (r * 2 + kv) * G + g; return pw[i][x >> 2][x & 3]; };
-      const bool whole = t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window);      // every column sees every token of the block
-      // scores
-      f32x4 sc[NT][2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) sc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          bf16x8_t kf[2];
-#pragma unroll
-          for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(kw[x >> 2][x & 3]); }
-#pragma unroll
-          for (int t = 0; t < NT; t++) {
-            f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-#pragma unroll
-              for (int term = 0; term < TERMS; term++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], qf[t][2 * g + c][term], d, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const unsigned int w = par(i, r, 0, g);
-              const float st = bf16_hi(w), z = fmaf(-128.f, st, bf16_lo(w));
-              sc[t][i][r] = fmaf(st, d[r], fmaf(z, qsum[t][g], sc[t][i][r]));
-            }
-          }
-        }
-      }
-      // weights
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        float mx = -INFINITY;
-        bool seen[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int j = t0 + 16 * i + 4 * q4 + r;
-            seen[i][r] = whole || (j <= my_pos[t] && (a.window <= 0 || j > my_pos[t] - a.window));
-            sc[t][i][r] *= a.scale_log2;
-            if (!seen[i][r]) sc[t][i][r] = -INFINITY;
-            mx = fmaxf(mx, sc[t][i][r]);
-          }
-        mx = kv4_max_quarters(mx);
-        // the sums keep their reference until a maximum passes it by 8 (weights up to 256 then): few blocks rescale
-        if (__any(mx > m[t] + 8.f)) {
-          const float nm = fmaxf(m[t], mx), f = nm > m[t] ? __builtin_amdgcn_exp2f(m[t] - nm) : 1.f;
-          m[t] = nm;
-          l[t] *= f;
-#pragma unroll
-          for (int g = 0; g < G; g++) lov[t][g] *= f;
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float fr = __shfl(f, 4 * q4 + r, 64);
-#pragma unroll
-            for (int c = 0; c < CT; c++) o[t][c][r] *= fr;
-#pragma unroll
-            for (int g = 0; g < G; g++) ones[t][g][r] *= fr;
-          }
-        }
-        float p[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            p[i][r] = seen[i][r] ? __builtin_amdgcn_exp2f(sc[t][i][r] - m[t]) : 0.f;
-            l[t] += p[i][r];
-          }
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          float ps[8];
-#pragma unroll
-          for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const unsigned int w = par(i, r, 1, g);
-              ps[4 * i + r] = seen[i][r] ? p[i][r] * bf16_hi(w) : 0.f;
-              lov[t][g] = seen[i][r] ? fmaf(p[i][r], bf16_lo(w), lov[t][g]) : lov[t][g];
-            }
-          u32x4 pf, pl;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            pf[e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
-            if constexpr (TERMS == 2) pl[e] = pack_bf16(ps[2 * e] - bf16_lo(pf[e]), ps[2 * e + 1] - bf16_hi(pf[e]));
-          }
-          const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, pf), pq = __builtin_bit_cast(bf16x8_t, pl);
-          ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ph, one8, ones[t][g], 0, 0, 0);
-          if constexpr (TERMS == 2) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pq, one8, ones[t][g], 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int x = 4 * g + c;
-            const bf16x8_t vf = kv4_frag(vw[x >> 2][x & 3]);
-            o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ph, vf, o[t][x], 0, 0, 0);
-            if constexpr (TERMS == 2) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pq, vf, o[t][x], 0, 0, 0);
-          }
-        }
-      }
+  const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+  unsigned int mask = 0x000f000fu, off = 0x43004300u;      // (in registers: one instruction a pair with both)
+  asm("" : "+s"(mask), "+v"(off));
+  // blocks of 32 from b on that are walked: those with a key that some column sees, on a page that is there
+  const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
+  auto next = [&](int b, const unsigned int*& blk) {
+    for (; b < b_hi; b += KW) {
+      const unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
+      if (page) { blk = page + (size_t)(b & 3) * kv4_block_words<HD>(); break; }
     }
+    return b;
+  };
+  Sums s;
+  Kv4Raw<HD> raw[2];
+  const unsigned int* blk = nullptr;
+  int b = next(b_lo + wv, blk);
+  if (b < b_hi) raw[0].load(blk, lane);
+  s.start(a, en, kvh, col0, ncol, q4, r16);
+  auto work = [&](const Kv4Raw<HD>& r, int bb) {
+    const int t0 = bb * KV4_BLK;
+    if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+    else s.template block<true>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+  };
+  while (b < b_hi) {
+    const int b1 = next(b + KW, blk);
+    if (b1 < b_hi) raw[1].load(blk, lane);
+    work(raw[0], b);
+    if (b1 >= b_hi) break;
+    b = next(b1 + KW, blk);
+    if (b < b_hi) raw[0].load(blk, lane);
+    work(raw[1], b1);
   }
-  // the columns' sums: o - 128 sum(weights) + lo part, denominators over the four quarters
+  s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    l[t] = kv4_sum_quarters(l[t]);
+    const int c0 = col0 + 16 * t, nv = min(16, ncol - c0);
+    if (nv <= 0) break;
+    if (t > 0) __syncthreads();
+    if (q4 == 0) { s_ml[wv][r16][0] = s.m[t]; s_ml[wv][r16][1] = s.l[t]; }
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-      const float lg = kv4_sum_quarters(lov[t][g]);
+    for (int r = 0; r < 4; r++) {
+      const int c = 4 * q4 + r;
+      if (c < nv)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float add = fmaf(-128.f, ones[t][g][r], __shfl(lg, 4 * q4 + r, 64));
+        for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + r16] = s.o[t][x][r];
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < nv * (HD / 4); item += 64 * KW) {
+      const int c = item / (HD / 4), x = item % (HD / 4);
+      float mx = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
+      for (int w = 0; w < KW; w++) mx = fmaxf(mx, s_ml[w][c][0]);
+      float den = 0.f;
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        const float mw = s_ml[w][c][0], f = mw == mx ? 1.f : __builtin_amdgcn_exp2f((mw - mx) * a.scale_log2);      // (all -inf: sums of zero)
+        const f32x4 v = *reinterpret_cast<const f32x4*>(kv4_lds + (w * nv + c) * HD + 4 * x);
+        den = fmaf(f, s_ml[w][c][1], den);
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(f, v[i], acc[i]);
+      }
+      const int col = c0 + c, i = en.count == 1 ? 0 : col / a.group, h = kvh * a.group + col - i * a.group;
+      if (a.splits > 1) {
+        const long long rec = ((en.tok0 + i) * a.heads + h) * a.splits + split;
+        *reinterpret_cast<f32x4*>(a.part + rec * HD + 4 * x) = acc;
+        if (x == 0) { a.ml[rec * 2] = mx; a.ml[rec * 2 + 1] = den; }
+      } else {
+        const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = round_storage_mode(acc[e] * inv, a.act16);
+        kv4_store4(a.out, (en.tok0 + i) * a.o_ts + h * a.o_hs + 4 * x, acc, a.q_dt);
       }
     }
   }
-  if constexpr (KW == 4) {
-    // the four waves' sums meet two and two: a lane's registers are the same places in every wave
-    __shared__ float so[2][NT][CT * 4][64], sm[2][NT][2][64];
-#pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {
-      __syncthreads();
-      if (wv >= half && wv < 2 * half) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          sm[wv - half][t][0][lane] = m[t]; sm[wv - half][t][1][lane] = l[t];
-#pragma unroll
-          for (int c = 0; c < CT; c++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) so[wv - half][t][c * 4 + r][lane] = o[t][c][r];
-        }
-      }
-      __syncthreads();
-      if (wv < half) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          const float m2 = sm[wv][t][0][lane], l2 = sm[wv][t][1][lane], nm = fmaxf(m[t], m2);
-          const float f1 = m[t] == nm ? 1.f : __builtin_amdgcn_exp2f(m[t] - nm), f2 = m2 == nm ? 1.f : __builtin_amdgcn_exp2f(m2 - nm);      // (both -inf: sums of zero)
-          m[t] = nm;
-          l[t] = l[t] * f1 + l2 * f2;
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float a1 = __shfl(f1, 4 * q4 + r, 64), a2 = __shfl(f2, 4 * q4 + r, 64);
-#pragma unroll
-            for (int c = 0; c < CT; c++) o[t][c][r] = o[t][c][r] * a1 + so[wv][t][c * 4 + r][lane] * a2;
-          }
-        }
-      }
+}
+
+// Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys.
+template <int HD, int NT, int TQ, int TP>
+__global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
+  typedef Kv4Sums<HD, NT, TQ, TP> Sums;
+  constexpr int CT = Sums::CT;
+  __shared__ __attribute__((aligned(16))) unsigned int s_par[4][HD];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q4 = lane >> 4, r16 = lane & 15;
+  const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  const int ncol = en.count * a.group, col0 = ((int)blockIdx.y * 4 + wv) * 16 * NT;
+  if (col0 >= ncol) return;      // (no barrier follows)
+  const int first = en.start + col0 / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;
+  const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
+  const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+  unsigned int mask = 0x000f000fu, off = 0x43004300u;
+  asm("" : "+s"(mask), "+v"(off));
+  const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
+  auto next = [&](int b, const unsigned int*& blk) {
+    for (; b < b_hi; b++) {
+      const unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
+      if (page) { blk = page + (size_t)(b & 3) * kv4_block_words<HD>(); break; }
     }
-    if (wv != 0) return;
+    return b;
+  };
+  Sums s;
+  Kv4Raw<HD> raw[2];
+  const unsigned int* blk = nullptr;
+  int b = next(b_lo, blk);
+  if (b < b_hi) raw[0].load(blk, lane);
+  s.start(a, en, kvh, col0, ncol, q4, r16);
+  auto work = [&](const Kv4Raw<HD>& r, int bb) {
+    const int t0 = bb * KV4_BLK;
+    if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+    else s.template block<true>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+  };
+  while (b < b_hi) {
+    const int b1 = next(b + 1, blk);
+    if (b1 < b_hi) raw[1].load(blk, lane);
+    work(raw[0], b);
+    if (b1 >= b_hi) break;
+    b = next(b1 + 1, blk);
+    if (b < b_hi) raw[0].load(blk, lane);
+    work(raw[1], b1);
   }
+  s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    if (a.splits > 1 && valid[t] && q4 == 0) {
-      const int c = col0 + 16 * t + r16;
-      const long long row = (en.tok0 + c / a.group) * a.heads + kvh * a.group + c % a.group;
-      a.ml[(row * a.splits + split) * 2] = m[t];
-      a.ml[(row * a.splits + split) * 2 + 1] = l[t];
+    const int mine = col0 + 16 * t + r16;
+    if (a.splits > 1 && mine < ncol && q4 == 0) {
+      const long long rec = ((en.tok0 + mine / a.group) * a.heads + kvh * a.group + mine % a.group) * a.splits + split;
+      a.ml[rec * 2] = s.m[t];
+      a.ml[rec * 2 + 1] = s.l[t];
     }
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const int c = col0 + 16 * t + 4 * q4 + r;
-      const float den = __shfl(l[t], 4 * q4 + r, 64);
+      const float den = __shfl(s.l[t], 4 * q4 + r, 64);
       if (c >= ncol) continue;
-      const int i = c / a.group, h = kvh * a.group + c % a.group;
+      const int i = c / a.group, h = kvh * a.group + c - i * a.group;
       if (a.splits > 1) {
         float* dst = a.part + (((en.tok0 + i) * a.heads + h) * a.splits + split) * HD;
 #pragma unroll
-        for (int x = 0; x < CT; x++) dst[16 * x + r16] = o[t][x][r];
+        for (int x = 0; x < CT; x++) dst[16 * x + r16] = s.o[t][x][r];
       } else {
-        const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
+        const float inv = den == 0.f ? 0.f : 1.f / den;
         const long long at = (en.tok0 + i) * a.o_ts + h * a.o_hs;
 #pragma unroll
-        for (int x = 0; x < CT; x++) kv4_store(a.out, at + 16 * x + r16, round_storage_mode(o[t][x][r] * inv, a.act16), a.q_dt);
+        for (int x = 0; x < CT; x++) kv4_store(a.out, at + 16 * x + r16, round_storage_mode(s.o[t][x][r] * inv, a.act16), a.q_dt);
       }
     }
   }
@@ -572,7 +723,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
     mx = group_max<64>(mx);
     float tot = 0.f;
     for (int s = tid; s < S; s += 64) {
-      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f(ms - mx);
+      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f((ms - mx) * a.scale_log2);
       sw[s] = w;
       tot += w * ml[2 * s + 1];
     }
@@ -599,7 +750,8 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
     const float inv = stot == 0.f ? 0.f : 1.f / stot;
     const long long at = (en.tok0 + blockIdx.y) * a.o_ts + h * a.o_hs + 4 * tid;
 #pragma unroll
-    for (int i = 0; i < 4; i++) kv4_store(a.out, at + i, round_storage_mode(acc[i] * inv, a.act16), a.q_dt);
+    for (int i = 0; i < 4; i++) acc[i] = round_storage_mode(acc[i] * inv, a.act16);
+    kv4_store4(a.out, at, acc, a.q_dt);
   }
 }
 

@@ -107,12 +107,13 @@ void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s) {
     else hipLaunchKernelGGL((tgx::kv4_read_kernel<128, DT>), grid, dim3(64), 0, s, a);)
 }
 
-template <int HD, int TERMS>
+template <int HD, int TQ, int TP, int TPC>
 static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
-  const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries), blk(256);
-  if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 1, 4, TERMS>), grid, blk, 0, s, a);
-  else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 2, 4, TERMS>), grid, blk, 0, s, a);
-  else hipLaunchKernelGGL((tgx::kv4_attend_kernel<HD, 2, 1, TERMS>), grid, blk, 0, s, a);
+  const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries);
+  const size_t lds = (size_t)p.kw * std::min<long long>(16, (long long)a.max_count * a.group) * HD * 4;
+  if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TPC>), grid, dim3(256), 0, s, a);
 }
 
 // a.splits, a.part, a.ml follow from the plan and the workspace here; with keys and values to append that the attention launch does not append itself, an append launch first
@@ -122,9 +123,16 @@ void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws,
   const size_t rows = (size_t)a.tokens * a.heads;
   a.splits = p.splits;
   a.part = ws; a.ml = ws + rows * p.splits * hd;
-  const bool two = a.q_dt != tgx::DT_BF16;
-  if (hd == 64) { if (two) launch_attend<64, 2>(a, p, s); else launch_attend<64, 1>(a, p, s); }
-  else { if (two) launch_attend<128, 2>(a, p, s); else launch_attend<128, 1>(a, p, s); }
+  // terms of queries and weights by the outputs' type (kernels/kv4.h)
+  if (hd == 64) {
+    if (a.q_dt == tgx::DT_BF16) launch_attend<64, 1, 2, 1>(a, p, s);
+    else if (a.q_dt == tgx::DT_F16) launch_attend<64, 2, 2, 2>(a, p, s);
+    else launch_attend<64, 3, 3, 3>(a, p, s);
+  } else {
+    if (a.q_dt == tgx::DT_BF16) launch_attend<128, 1, 2, 1>(a, p, s);
+    else if (a.q_dt == tgx::DT_F16) launch_attend<128, 2, 2, 2>(a, p, s);
+    else launch_attend<128, 3, 3, 3>(a, p, s);
+  }
   if (p.splits > 1) {
     const dim3 grid(a.heads, a.max_count, a.entries);
     if (hd == 64) hipLaunchKernelGGL(tgx::kv4_combine_kernel<64>, grid, dim3(256), 0, s, a);
@@ -207,7 +215,7 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   if (k && (rc = check_kv(k, v, a))) return rc;
   if (!std::isfinite(scale)) return op_err(TGX_ERR_INVALID, "scale is not finite");
   a.q = q->data; a.out = out->data; a.q_dt = kv4_dt(q->dtype); a.q_ts = q->token_stride; a.q_hs = q->head_stride; a.o_ts = out->token_stride; a.o_hs = out->head_stride;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  tgx::kv4_scale(a, scale);
   if (!a.max_count || !a.tokens) return TGX_OK;
   OnDevice on(device);
   if (on.rc) return on.rc;

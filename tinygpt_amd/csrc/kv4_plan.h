@@ -24,7 +24,8 @@ struct Kv4Args {
   void *k, *v; int kv_dt; long long k_ts, k_hs, v_ts, v_hs, slot_s;
   // attention
   const void* q; void* out; int q_dt; long long q_ts, q_hs, o_ts, o_hs;
-  int heads, group; float scale_log2;                         // score scale * log2(e)
+  int heads, group;
+  float scale_log2, q_sign, gap;                              // |score scale| * log2(e) (1 for a scale of 0), the scale's sign, 8 / scale_log2: see kv4_scale
   int window;                                                 // > 0: position p sees keys p - window + 1 .. p
   int splits; float *part, *ml;                               // splits > 1: [token * heads + head][splits][HD] sums, [..][splits][2] (maximum, denominator)
   int act16;                                                  // outputs rounded to the storage type: 0 no, 1 bf16, 2 fp16 (option act.round16 of a model)
@@ -62,6 +63,13 @@ TGX_KV4 int kv4_key_bit(int ch) { return kv4_code_bit(ch & 7); }
 TGX_KV4 int kv4_value_bit(int t) { return kv4_code_bit((t & 3) + 4 * ((t >> 4) & 1)); }
 TGX_KV4 int kv4_value_token(int q, int e) { return e < 4 ? 4 * q + e : 12 + 4 * q + e; }      // the token of a value word's code e
 
+// A scale enters as a positive factor of the scores and a sign of the queries (0: queries of zero), so that the largest score is the largest before the scale
+inline void kv4_scale(Kv4Args& a, float scale) {
+  a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+  a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  a.gap = std::min(8.f / a.scale_log2, 1e30f);
+}
+
 // pages [lo, hi) that split `split` of `splits` walks for columns at positions first .. last
 struct Kv4Range { int lo, hi; };
 TGX_KV4 Kv4Range kv4_range(int first, int last, int window, int table_len, int split, int splits) {
@@ -72,20 +80,21 @@ TGX_KV4 Kv4Range kv4_range(int first, int last, int window, int table_len, int s
   return Kv4Range{(int)(p0 < hi ? p0 : hi), (int)(p1 < hi ? p1 : hi)};
 }
 
-// How a batch's attention is divided: kw 4 = the waves of a workgroup share nt * 16 columns (token, query head) and divide the keys, kw 1 = they divide the columns;
+// How a batch's attention is divided: kw > 1 = the kw waves of a workgroup share nt * 16 columns (token, query head) and divide the keys, kw 1 = four waves divide the columns;
 // tiles workgroups of columns, splits of the keys between workgroups
 struct Kv4Plan { int kw, nt, tiles, splits; };
 inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int window, long long max_keys, int num_cus) {
   Kv4Plan p;
   const long long cols = (long long)max_count * group;
   p.kw = cols <= 32 ? 4 : 1;
-  p.nt = p.kw == 4 ? (cols <= 16 ? 1 : 2) : 2;
-  const int per = 16 * p.nt * (p.kw == 4 ? 1 : 4);
+  p.nt = p.kw > 1 ? (cols <= 16 ? 1 : 2) : 2;
+  const int per = 16 * p.nt * (p.kw > 1 ? 1 : 4);
   p.tiles = (int)((cols + per - 1) / per);
   const long long keys = window > 0 ? std::min<long long>(max_keys, (long long)window + max_count) : max_keys;
   const long long pages = std::max<long long>(1, (keys + KV4_PAGE - 1) / KV4_PAGE);
   const long long wgs = std::max<long long>(1, (long long)entries * kv_heads * p.tiles);
-  p.splits = (int)std::max<long long>(1, std::min<long long>({(4ll * num_cus + wgs - 1) / wgs, pages, 256}));
+  const long long want = ((p.kw > 1 ? 4ll : 1ll) * num_cus + wgs - 1) / wgs;
+  p.splits = (int)std::max<long long>(1, std::min<long long>({want, pages, 256}));
   return p;
 }
 inline size_t kv4_part_floats(const Kv4Plan& p, long long rows, int hd) { return p.splits > 1 ? (size_t)rows * p.splits * (hd + 2) : 0; }      // workspace of the splits' records

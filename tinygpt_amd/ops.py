@@ -46,6 +46,7 @@ class Kv4Cache:
             raise ValueError(f"pool ({pool.device}) and table ({table.device}) are on one GPU")
         self.pool, self.table, self.kv_heads, self.head_dim = pool, table, kv_heads, head_dim
         self.device = pool.device
+        self._rows_of = {kv_heads: (kv_heads, head_dim)}
         self._layer_bytes = pool.shape[1] * nbytes
         stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
         if stride < table.shape[1]:
