@@ -280,13 +280,25 @@ __device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w, unsigned int mask, 
   for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & mask) | off;
   return __builtin_bit_cast(bf16x8_t, f);
 }
-__device__ __forceinline__ float kv4_max_quarters(float v) {      // over the lanes of equal r
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+// over the lanes of equal r: lanes 16 and 32 further swap in the vector registers
+__device__ __forceinline__ float kv4_max_quarters(float v) {
+  u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+  w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 __device__ __forceinline__ float kv4_sum_quarters(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  v = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+  w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+// the page of a block, -1: none.  Tables are read through the scalar cache: an entry in front of its use costs no vector register and waits for no vector load
+__device__ __forceinline__ int kv4_page_id(const Kv4Args& a, int seq, int b, int b_hi) {
+  if (b >= b_hi || (b >> 2) >= a.table_len) return -1;
+  const int* at = a.table + (long long)seq * a.table_stride + (b >> 2);
+  const int p = *(const __attribute__((address_space(4))) int*)at;
+  return p >= 0 && p < a.pages ? p : -1;
 }
 // eight neighbouring channels of a row of a runtime type
 __device__ __forceinline__ void kv4_load8(const void* p, long long i, int dt, float x[8]) {
@@ -539,7 +551,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   extern __shared__ __attribute__((aligned(16))) float kv4_lds[];
   __shared__ __attribute__((aligned(16))) unsigned int s_par[KW][HD];
   __shared__ float s_ml[KW][16][2];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q4 = lane >> 4, r16 = lane & 15;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
   const int ncol = en.count * a.group, col0 = (int)blockIdx.y * 16 * NT;
@@ -560,32 +572,23 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   asm("" : "+s"(mask), "+v"(off));
   // blocks of 32 from b on that are walked: those with a key that some column sees, on a page that is there
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
-  auto next = [&](int b, const unsigned int*& blk) {
-    for (; b < b_hi; b += KW) {
-      const unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
-      if (page) { blk = page + (size_t)(b & 3) * kv4_block_words<HD>(); break; }
-    }
-    return b;
-  };
+  // the blocks b_lo + wv, .. in steps of KW: one on its way while one is worked on, the page of the one behind on its way before that
   Sums s;
-  Kv4Raw<HD> raw[2];
-  const unsigned int* blk = nullptr;
-  int b = next(b_lo + wv, blk);
-  if (b < b_hi) raw[0].load(blk, lane);
+  Kv4Raw<HD> raw, nxt;
+  int b = b_lo + wv, id = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + KW, b_hi);
+  const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
+  const size_t page_words = (size_t)a.kv_heads * (36 * HD);
+  if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  auto work = [&](const Kv4Raw<HD>& r, int bb) {
-    const int t0 = bb * KV4_BLK;
-    if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-    else s.template block<true>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-  };
-  while (b < b_hi) {
-    const int b1 = next(b + KW, blk);
-    if (b1 < b_hi) raw[1].load(blk, lane);
-    work(raw[0], b);
-    if (b1 >= b_hi) break;
-    b = next(b1 + KW, blk);
-    if (b < b_hi) raw[0].load(blk, lane);
-    work(raw[1], b1);
+  for (; b < b_hi; b += KW) {
+    const int id2 = kv4_page_id(a, en.seq, b + 2 * KW, b_hi);
+    if (id1 >= 0) nxt.load(heads + id1 * page_words + (size_t)((b + KW) & 3) * kv4_block_words<HD>(), lane);
+    if (id >= 0) {
+      const int t0 = b * KV4_BLK;
+      if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+      else s.template block<true>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+    }
+    raw = nxt; id = id1; id1 = id2;
   }
   s.finish(q4);
 #pragma unroll
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
   __shared__ __attribute__((aligned(16))) unsigned int s_par[4][HD];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q4 = lane >> 4, r16 = lane & 15;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
   const int ncol = en.count * a.group, col0 = ((int)blockIdx.y * 4 + wv) * 16 * NT;
@@ -649,32 +652,23 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
   unsigned int mask = 0x000f000fu, off = 0x43004300u;
   asm("" : "+s"(mask), "+v"(off));
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
-  auto next = [&](int b, const unsigned int*& blk) {
-    for (; b < b_hi; b++) {
-      const unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
-      if (page) { blk = page + (size_t)(b & 3) * kv4_block_words<HD>(); break; }
-    }
-    return b;
-  };
+  // the blocks b_lo, .. one by one: one on its way while one is worked on, the page of the one behind on its way before that
   Sums s;
-  Kv4Raw<HD> raw[2];
-  const unsigned int* blk = nullptr;
-  int b = next(b_lo, blk);
-  if (b < b_hi) raw[0].load(blk, lane);
+  Kv4Raw<HD> raw, nxt;
+  int b = b_lo, id = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + 1, b_hi);
+  const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
+  const size_t page_words = (size_t)a.kv_heads * (36 * HD);
+  if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  auto work = [&](const Kv4Raw<HD>& r, int bb) {
-    const int t0 = bb * KV4_BLK;
-    if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-    else s.template block<true>(r, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-  };
-  while (b < b_hi) {
-    const int b1 = next(b + 1, blk);
-    if (b1 < b_hi) raw[1].load(blk, lane);
-    work(raw[0], b);
-    if (b1 >= b_hi) break;
-    b = next(b1 + 1, blk);
-    if (b < b_hi) raw[0].load(blk, lane);
-    work(raw[1], b1);
+  for (; b < b_hi; b += 1) {
+    const int id2 = kv4_page_id(a, en.seq, b + 2 * 1, b_hi);
+    if (id1 >= 0) nxt.load(heads + id1 * page_words + (size_t)((b + 1) & 3) * kv4_block_words<HD>(), lane);
+    if (id >= 0) {
+      const int t0 = b * KV4_BLK;
+      if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+      else s.template block<true>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
+    }
+    raw = nxt; id = id1; id1 = id2;
   }
   s.finish(q4);
 #pragma unroll
