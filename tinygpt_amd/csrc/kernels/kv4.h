@@ -402,8 +402,8 @@ struct Kv4Sums {
     }
   }
 
-  // one block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters (which every lane needs of the four tokens of its scores).  MASK: some column does not see
-  // some token of the block; what is not seen is selected away, whatever it holds.
+  // One block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters, which every lane needs of the four tokens of its scores.  MASK: some column does not
+  // see some token of the block; what is not seen is selected away, whatever it holds.  In phases that the compiler does not mix: mixed, their registers are half again as many.
   template <bool MASK>
   __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
     const int q4 = lane >> 4;
@@ -411,17 +411,21 @@ struct Kv4Sums {
     if constexpr (PW == 4) *reinterpret_cast<u32x4*>(sp + (lane & 31) * 4) = u32x4{raw.p[0], raw.p[1], raw.p[2], raw.p[3]};
     else *reinterpret_cast<u32x2*>(sp + (lane & 31) * 2) = u32x2{raw.p[0], raw.p[1]};
     wave_fence();
-    unsigned int par[2][4][PW];
+    // the keys' (which 0) or the values' (1) parameters of a lane's tokens
+    auto parameters = [&](unsigned int (&par)[2][4][G], int which) {
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int r = 0; r < 4; r++)
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int w = 0; w < PW; w++) par[i][r][w] = sp[(16 * i + 4 * q4 + r) * PW + w];
-    wave_fence();
+          for (int g = 0; g < G; g++) par[i][r][g] = sp[(16 * i + 4 * q4 + r) * PW + which * G + g];
+    };
+    unsigned int par[2][4][G];
+    parameters(par, 0);
     f32x4 sc[NT][2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < G; g++) {
         bf16x8_t kf[2];
@@ -442,18 +446,18 @@ struct Kv4Sums {
         }
       }
     }
-    u32x4 pf[NT][G][TP];
+    float p[NT][2][4];
+    bool seen[NT][2][4];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      bool seen[2][4];
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           const int j = t0 + 16 * i + 4 * q4 + r;
-          seen[i][r] = !MASK || (j <= pos[t] && (window <= 0 || j > pos[t] - window));
-          if (MASK && !seen[i][r]) sc[t][i][r] = -INFINITY;
+          seen[t][i][r] = !MASK || (j <= pos[t] && (window <= 0 || j > pos[t] - window));
+          if (MASK && !seen[t][i][r]) sc[t][i][r] = -INFINITY;
           mx = fmaxf(mx, sc[t][i][r]);
         }
       mx = kv4_max_quarters(mx);
@@ -474,43 +478,44 @@ struct Kv4Sums {
         }
       }
       const float ref = -m[t] * scale;
-      float p[2][4];
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          p[i][r] = __builtin_amdgcn_exp2f(fmaf(sc[t][i][r], scale, ref));
-          if (MASK && !seen[i][r]) p[i][r] = 0.f;
-          l[t] += p[i][r];
+          p[t][i][r] = __builtin_amdgcn_exp2f(fmaf(sc[t][i][r], scale, ref));
+          if (MASK && !seen[t][i][r]) p[t][i][r] = 0.f;
+          l[t] += p[t][i][r];
         }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    parameters(par, 1);
+    wave_fence();
+    const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
-      for (int g = 0; g < G; g++) {
+    for (int g = 0; g < G; g++) {
+      u32x4 pf[NT][TP];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
         float ps[8];
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const unsigned int w = par[i][r][G + g];
+            const unsigned int w = par[i][r][g];
             const float st = bf16_hi(w), lo = CENTRE ? fmaf(8.f, st, bf16_lo(w)) : bf16_lo(w);
-            ps[4 * i + r] = MASK && !seen[i][r] ? 0.f : p[i][r] * st;
-            lov[t][g] = MASK && !seen[i][r] ? lov[t][g] : fmaf(p[i][r], lo, lov[t][g]);
+            ps[4 * i + r] = MASK && !seen[t][i][r] ? 0.f : p[t][i][r] * st;
+            lov[t][g] = MASK && !seen[t][i][r] ? lov[t][g] : fmaf(p[t][i][r], lo, lov[t][g]);
           }
 #pragma unroll
         for (int term = 0; term < TP; term++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            pf[t][g][term][e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
-            if (term + 1 < TP) { ps[2 * e] -= bf16_lo(pf[t][g][term][e]); ps[2 * e + 1] -= bf16_hi(pf[t][g][term][e]); }
+            pf[t][term][e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
+            if (term + 1 < TP) { ps[2 * e] -= bf16_lo(pf[t][term][e]); ps[2 * e + 1] -= bf16_hi(pf[t][term][e]); }
           }
+#pragma unroll
+        for (int term = 0; term < TP; term++) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][term]), one8, ones[t][g], 0, 0, 0);
       }
-    }
-    const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int term = 0; term < TP; term++) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][g][term]), one8, ones[t][g], 0, 0, 0);
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const int x = 4 * g + c;
@@ -518,9 +523,40 @@ struct Kv4Sums {
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int term = 0; term < TP; term++) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][g][term]), vf, o[t][x], 0, 0, 0);
+          for (int term = 0; term < TP; term++) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][term]), vf, o[t][x], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  }
+
+  // The blocks b0, b0 + STEP, .. below b1, every one (MASK false) or only those of them outside of [skip0, skip1) (MASK true): one on its way while one is worked on, the page of the one behind on its way
+  // before that.  A walk takes one kind of block: with both in one loop the compiler keeps two sets of sums.
+  template <bool MASK, int STEP>
+  __device__ __forceinline__ void walk(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+    const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
+    const size_t page_words = (size_t)a.kv_heads * (36 * HD);
+    auto past = [&](int b) { return MASK && b >= skip0 && b < skip1 ? b + (skip1 - b + STEP - 1) / STEP * STEP : b; };
+    Kv4Raw<HD> raw, nxt;
+    int b = past(b0), bn = past(b + STEP), id = kv4_page_id(a, seq, b, b1), idn = kv4_page_id(a, seq, bn, b1);
+    if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
+    while (b < b1) {
+      const int bm = past(bn + STEP), idm = kv4_page_id(a, seq, bm, b1);
+      if (idn >= 0) nxt.load(heads + idn * page_words + (size_t)(bn & 3) * kv4_block_words<HD>(), lane);
+      if (id >= 0) block<MASK>(raw, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane, mask, off);
+      raw = nxt; b = bn; id = idn; bn = bm; idn = idm;
+    }
+  }
+  // a wave's blocks (b_lo + first, in steps) of columns at positions p0 .. p1: those that every column sees whole, then the others
+  template <int STEP>
+  __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+    // whole for every column: t0 + 31 <= p0 and t0 > p1 - window
+    int w1 = (p0 + 1) >> 5, w0 = a.window > 0 && p1 - a.window + 1 > 0 ? (p1 - a.window + KV4_BLK) >> 5 : 0;
+    w1 = min(max(w1, 0), b_hi);
+    w0 = min(w0, w1);
+    int f = first_block;
+    if (f < w0) f += (w0 - f + STEP - 1) / STEP * STEP;
+    walk<false, STEP>(a, seq, kvh, f, w1, 0, 0, sp, lane, mask, off);
+    walk<true, STEP>(a, seq, kvh, first_block, b_hi, w0, w1, sp, lane, mask, off);
   }
 
   // o becomes the columns' sums, l their denominators (over the four quarters)
@@ -542,8 +578,52 @@ struct Kv4Sums {
   }
 };
 
-// Few columns (a token's query heads, or a few tokens'): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
-// The next block is on its way while one is worked on.  The waves' sums meet once in LDS, where a thread takes four channels of a column through all waves.
+// The waves' sums of up to 16 columns meet in LDS: so [KW][columns][HD], a thread takes four channels of a column through all waves; the split's record, or the output.
+template <int HD, int KW>
+__device__ __forceinline__ void kv4_meet(const Kv4Args& a, const Kv4Entry& en, int kvh, int split, int c0, int nv, const float* so, const float (*s_ml)[16][2]) {
+  for (int item = threadIdx.x; item < nv * (HD / 4); item += 64 * KW) {
+    const int c = item / (HD / 4), x = item % (HD / 4);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < KW; w++) mx = fmaxf(mx, s_ml[w][c][0]);
+    float den = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+      const float mw = s_ml[w][c][0], f = mw == mx ? 1.f : __builtin_amdgcn_exp2f((mw - mx) * a.scale_log2);      // (all -inf: sums of zero)
+      const f32x4 v = *reinterpret_cast<const f32x4*>(so + (w * nv + c) * HD + 4 * x);
+      den = fmaf(f, s_ml[w][c][1], den);
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[i] = fmaf(f, v[i], acc[i]);
+    }
+    const int col = c0 + c, i = en.count == 1 ? 0 : col / a.group, h = kvh * a.group + col - i * a.group;
+    if (a.splits > 1) {
+      const long long rec = ((en.tok0 + i) * a.heads + h) * a.splits + split;
+      *reinterpret_cast<f32x4*>(a.part + rec * HD + 4 * x) = acc;
+      if (x == 0) { a.ml[rec * 2] = mx; a.ml[rec * 2 + 1] = den; }
+    } else {
+      const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[e] = round_storage_mode(acc[e] * inv, a.act16);
+      kv4_store4(a.out, (en.tok0 + i) * a.o_ts + h * a.o_hs + 4 * x, acc, a.q_dt);
+    }
+  }
+}
+
+// a single token's key and value join the cache, by the workgroup whose pages hold its place; every thread of it comes here
+template <int HD>
+__device__ __forceinline__ void kv4_append_first(const Kv4Args& a, const Kv4Entry& en, const Kv4Range& rg, int kvh) {
+  if (a.k != nullptr && en.count == 1 && en.start >= 0) {
+    const int b = en.start >> KV4_PAGE_SHIFT;
+    if (b >= rg.lo && b < rg.hi) {
+      unsigned int* page = kv4_page(a, en.seq, b, kvh, HD);
+      if (page && threadIdx.x < 64) kv4_append_one<HD, true>(a, page, en.tok0, en.start, kvh);
+      __syncthreads();
+    }
+  }
+}
+
+// Few columns (a few tokens' query heads): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
 template <int HD, int NT, int KW, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
@@ -556,40 +636,16 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
   const int ncol = en.count * a.group, col0 = (int)blockIdx.y * 16 * NT;
   if (col0 >= ncol) return;
-  const int first = en.start + (en.count == 1 ? 0 : col0 / a.group), last = en.start + (en.count == 1 ? 0 : min(col0 + 16 * NT - 1, ncol - 1) / a.group);      // positions of the columns
+  const int first = en.start + col0 / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;      // positions of the columns
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
-  // this token's key and value first, by the workgroup whose pages hold its place (single tokens)
-  if (NT == 1 && a.k != nullptr && en.count == 1 && en.start >= 0) {
-    const int b = en.start >> KV4_PAGE_SHIFT;
-    if (b >= rg.lo && b < rg.hi) {
-      unsigned int* page = kv4_page(a, en.seq, b, kvh, HD);
-      if (page && wv == 0) kv4_append_one<HD, true>(a, page, en.tok0, en.start, kvh);
-      __syncthreads();
-    }
-  }
+  if (NT == 1) kv4_append_first<HD>(a, en, rg, kvh);
   const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   unsigned int mask = 0x000f000fu, off = 0x43004300u;      // (in registers: one instruction a pair with both)
   asm("" : "+s"(mask), "+v"(off));
-  // blocks of 32 from b on that are walked: those with a key that some column sees, on a page that is there
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
-  // the blocks b_lo + wv, .. in steps of KW: one on its way while one is worked on, the page of the one behind on its way before that
   Sums s;
-  Kv4Raw<HD> raw, nxt;
-  int b = b_lo + wv, id = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + KW, b_hi);
-  const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
-  const size_t page_words = (size_t)a.kv_heads * (36 * HD);
-  if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  for (; b < b_hi; b += KW) {
-    const int id2 = kv4_page_id(a, en.seq, b + 2 * KW, b_hi);
-    if (id1 >= 0) nxt.load(heads + id1 * page_words + (size_t)((b + KW) & 3) * kv4_block_words<HD>(), lane);
-    if (id >= 0) {
-      const int t0 = b * KV4_BLK;
-      if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-      else s.template block<true>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-    }
-    raw = nxt; id = id1; id1 = id2;
-  }
+  s.template all<KW>(a, en.seq, kvh, b_lo + wv, b_hi, first, last, s_par[wv], lane, mask, off);
   s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -605,33 +661,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
         for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + r16] = s.o[t][x][r];
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < nv * (HD / 4); item += 64 * KW) {
-      const int c = item / (HD / 4), x = item % (HD / 4);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < KW; w++) mx = fmaxf(mx, s_ml[w][c][0]);
-      float den = 0.f;
-      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < KW; w++) {
-        const float mw = s_ml[w][c][0], f = mw == mx ? 1.f : __builtin_amdgcn_exp2f((mw - mx) * a.scale_log2);      // (all -inf: sums of zero)
-        const f32x4 v = *reinterpret_cast<const f32x4*>(kv4_lds + (w * nv + c) * HD + 4 * x);
-        den = fmaf(f, s_ml[w][c][1], den);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(f, v[i], acc[i]);
-      }
-      const int col = c0 + c, i = en.count == 1 ? 0 : col / a.group, h = kvh * a.group + col - i * a.group;
-      if (a.splits > 1) {
-        const long long rec = ((en.tok0 + i) * a.heads + h) * a.splits + split;
-        *reinterpret_cast<f32x4*>(a.part + rec * HD + 4 * x) = acc;
-        if (x == 0) { a.ml[rec * 2] = mx; a.ml[rec * 2 + 1] = den; }
-      } else {
-        const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[e] = round_storage_mode(acc[e] * inv, a.act16);
-        kv4_store4(a.out, (en.tok0 + i) * a.o_ts + h * a.o_hs + 4 * x, acc, a.q_dt);
-      }
-    }
+    kv4_meet<HD, KW>(a, en, kvh, split, c0, nv, kv4_lds, s_ml);
   }
 }
 
@@ -652,24 +682,9 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
   unsigned int mask = 0x000f000fu, off = 0x43004300u;
   asm("" : "+s"(mask), "+v"(off));
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
-  // the blocks b_lo, .. one by one: one on its way while one is worked on, the page of the one behind on its way before that
   Sums s;
-  Kv4Raw<HD> raw, nxt;
-  int b = b_lo, id = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + 1, b_hi);
-  const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
-  const size_t page_words = (size_t)a.kv_heads * (36 * HD);
-  if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  for (; b < b_hi; b += 1) {
-    const int id2 = kv4_page_id(a, en.seq, b + 2 * 1, b_hi);
-    if (id1 >= 0) nxt.load(heads + id1 * page_words + (size_t)((b + 1) & 3) * kv4_block_words<HD>(), lane);
-    if (id >= 0) {
-      const int t0 = b * KV4_BLK;
-      if (t0 + KV4_BLK - 1 <= first && (a.window <= 0 || t0 > last - a.window)) s.template block<false>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-      else s.template block<true>(raw, t0, a.window, a.scale_log2, a.gap, s_par[wv], lane, mask, off);
-    }
-    raw = nxt; id = id1; id1 = id2;
-  }
+  s.template all<1>(a, en.seq, kvh, b_lo, b_hi, first, last, s_par[wv], lane, mask, off);
   s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -697,6 +712,249 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
       }
     }
   }
+}
+
+// Single tokens of up to RPT query heads a key / value head (4 or 8).  S = Q K^T the other way round: rows query heads, columns tokens, and the 16 rows are the heads 16 / RPT times
+// over, so that the products of 16 / RPT tiles of tokens give every lane the scores of one token for four heads (quarter q takes its rows from the product of tile q, or q / 2): a lane
+// reads the parameters of its own token, and each score, exponential and weight is worked out once and not for 16 columns of which RPT are asked for.  The weights
+// pass through LDS into the A operand of P V (rows heads).  What a row's four heads share (references, their sums' factors) is the same in every lane that holds the row.
+template <int HD, int RPT, int KW, int TQ, int TP>
+__global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args a) {
+  constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64, PW = HD / 32;
+  constexpr int NJ = 16 / RPT, TOK = 16 * NJ, NB = TOK / 32;      // tiles, tokens and blocks of a step
+  constexpr int WS = TOK + 8;                                     // a head's weights in LDS, padded by 16 bytes
+  extern __shared__ __attribute__((aligned(16))) float kv4_lds[];
+  __shared__ __attribute__((aligned(16))) unsigned short s_w[KW][TP][RPT][WS];      // one group's weights, in the order of the value words' tokens
+  __shared__ float s_ml[KW][16][2];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, n16 = lane & 15;
+  const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  if (en.count < 1) return;
+  const int last = en.start;
+  const Kv4Range rg = kv4_range(last, last, a.window, a.table_len, split, a.splits);
+  kv4_append_first<HD>(a, en, rg, kvh);
+  const int key_lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
+  unsigned int mask = 0x000f000fu, off = 0x43004300u;
+  asm("" : "+s"(mask), "+v"(off));
+  const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5) & ~(NB - 1);      // (a step's blocks are of one page)
+  const int tile = RPT == 4 ? q4 : q4 >> 1;                       // this lane's token of a step: 16 tile + n16, heads h0 .. h0 + 3
+  const int h0 = RPT == 4 ? 0 : 4 * (q4 & 1);
+  struct Raw { u32x4 k[NB][PARTS], v[NB][PARTS]; unsigned int p[PW]; };
+  const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
+  const size_t page_words = (size_t)a.kv_heads * (36 * HD);
+  auto load = [&](Raw& raw, int id, int b) {
+    const unsigned int* blk = heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>();
+#pragma unroll
+    for (int x = 0; x < NB; x++)
+#pragma unroll
+      for (int i = 0; i < PARTS; i++) raw.k[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>()) + i * 64 + lane);
+    const unsigned int* pw = blk + (tile >> 1) * kv4_block_words<HD>() + 8 * HD + (16 * (tile & 1) + n16) * PW;
+    if constexpr (PW == 4) { const u32x4 w = load_nt(reinterpret_cast<const u32x4*>(pw)); raw.p[0] = w[0]; raw.p[1] = w[1]; raw.p[2] = w[2]; raw.p[3] = w[3]; }
+    else { const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(pw)); raw.p[0] = w[0]; raw.p[1] = w[1]; }
+#pragma unroll
+    for (int x = 0; x < NB; x++)
+#pragma unroll
+      for (int i = 0; i < PARTS; i++) raw.v[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>() + 4 * HD) + i * 64 + lane);
+  };
+  constexpr int STEP = KW * NB;
+  Raw raw[2] = {};                                                // (codes of no block are numbers too)
+  int b = b_lo + wv * NB, id0 = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + STEP, b_hi);
+  if (id0 >= 0) load(raw[0], id0, b);
+  // queries: row n16 = head n16 % RPT, channels 32 c + 8 q .. + 7; the sums of a group's channels per head of this lane
+  bf16x8_t qf[CH][TQ];
+  float qs[G][4];
+  {
+    const long long base = en.tok0 * a.q_ts + (kvh * a.group + min(n16 % RPT, a.group - 1)) * a.q_hs + 8 * q4;
+    float sum[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) sum[g] = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < CH; ch++) {
+      float x[8];
+      kv4_load8(a.q, base + 32 * ch, a.q_dt, x);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
+#pragma unroll
+      for (int term = 0; term < TQ; term++) {
+        u32x4 f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          f[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+          sum[ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
+          x[2 * e] -= bf16_lo(f[e]); x[2 * e + 1] -= bf16_hi(f[e]);
+        }
+        qf[ch][term] = __builtin_bit_cast(bf16x8_t, f);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const float t = kv4_sum_quarters(sum[g]);
+#pragma unroll
+      for (int r = 0; r < 4; r++) qs[g][r] = __shfl(t, h0 + r, 64);
+    }
+  }
+  f32x4 o[CT], ones[G];
+  float m[4], ref[4], l[4], lov[G][4];                            // references of the weights, in scores before the scale and (ref) negative behind it
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    m[r] = -INFINITY; ref[r] = INFINITY; l[r] = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) lov[g][r] = 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < CT; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < G; g++) ones[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  const int w_at = (tile >> 1) * 32 + (n16 >> 2) * 8 + (n16 & 3) + 4 * (tile & 1);      // this lane's token among a head's weights
+  const float scale = a.scale_log2, gap = a.gap;
+
+  // one step: NB blocks from block bb on; what is not seen (or there) has levels of zero and a score of -inf
+  auto step = [&](const Raw& rw, int bb, bool there) {
+    const int j = bb * KV4_BLK + 16 * tile + n16;
+    const bool in = there && j >= key_lo && j <= last;
+    float st[2][G], lo[2][G];
+#pragma unroll
+    for (int w = 0; w < PW; w++) {
+      const unsigned int x = in ? rw.p[w] : 0u;
+      st[w / G][w % G] = bf16_hi(x); lo[w / G][w % G] = bf16_lo(x);
+    }
+    const float begin = in ? 0.f : -INFINITY;
+    float sc[4];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      f32x4 d[NJ];
+#pragma unroll
+      for (int t = 0; t < NJ; t++) {
+        d[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const int x = (t & 1) * CH + 2 * g + c;
+          const bf16x8_t kf = kv4_frag(rw.k[t >> 1][x >> 2][x & 3], mask, off);
+#pragma unroll
+          for (int term = 0; term < TQ; term++) d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[2 * g + c][term], kf, d[t], 0, 0, 0);
+        }
+      }
+      const float z = fmaf(-128.f, st[0][g], lo[0][g]);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        float v;
+        if constexpr (RPT == 4) v = q4 < 2 ? (q4 == 0 ? d[0][r] : d[1][r]) : (q4 == 2 ? d[NJ - 2][r] : d[NJ - 1][r]);
+        else v = q4 < 2 ? d[0][r] : d[1][r];
+        sc[r] = fmaf(st[0][g], v, fmaf(z, qs[g][r], g == 0 ? begin : sc[r]));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(sc[0] > m[0] + gap || sc[1] > m[1] + gap || sc[2] > m[2] + gap || sc[3] > m[3] + gap)) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        float mx = fmaxf(sc[r], m[r]);
+        mx = fmaxf(mx, dpp_mov<0xB1, 0xf>(mx));
+        mx = fmaxf(mx, dpp_mov<0x4E, 0xf>(mx));
+        mx = fmaxf(mx, dpp_mov<0x141, 0xf>(mx));
+        mx = fmaxf(mx, dpp_mov<0x140, 0xf>(mx));
+        u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false));
+        mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        if constexpr (RPT == 4) {
+          w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false));
+          mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        }
+        const float f = mx > m[r] ? __builtin_amdgcn_exp2f((m[r] - mx) * scale) : 1.f;
+        m[r] = mx; ref[r] = -mx * scale;
+        l[r] *= f;
+#pragma unroll
+        for (int g = 0; g < G; g++) { lov[g][r] *= f; ones[g][r] *= f; }
+#pragma unroll
+        for (int c = 0; c < CT; c++) o[c][r] *= f;
+      }
+    }
+    float p[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], scale, ref[r]));
+      if (!in) p[r] = 0.f;                                        // (a reference of -inf: nothing was seen yet)
+      l[r] += p[r];
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float ps[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) { ps[r] = p[r] * st[1][g]; lov[g][r] = fmaf(p[r], lo[1][g], lov[g][r]); }
+#pragma unroll
+      for (int term = 0; term < TP; term++) {
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const unsigned int w = pack_bf16(ps[r], ps[r + 1]);
+          s_w[wv][term][h0 + r][w_at] = (unsigned short)w;
+          s_w[wv][term][h0 + r + 1][w_at] = (unsigned short)(w >> 16);
+          if (term + 1 < TP) { ps[r] -= bf16_lo(w); ps[r + 1] -= bf16_hi(w); }
+        }
+      }
+      wave_fence();
+      bf16x8_t wf[NB][TP];
+#pragma unroll
+      for (int x = 0; x < NB; x++)
+#pragma unroll
+        for (int term = 0; term < TP; term++) wf[x][term] = *reinterpret_cast<const bf16x8_t*>(&s_w[wv][term][n16 % RPT][32 * x + 8 * q4]);
+      wave_fence();
+#pragma unroll
+      for (int x = 0; x < NB; x++) {
+#pragma unroll
+        for (int term = 0; term < TP; term++) ones[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], one8, ones[g], 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int i = 4 * g + c;
+          const bf16x8_t vf = kv4_frag(rw.v[x][i >> 2][i & 3], mask, off);
+#pragma unroll
+          for (int term = 0; term < TP; term++) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], vf, o[i], 0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // one step on its way while one is worked on, the page of the one behind on its way before that; no branch but the loop's around the sums
+  while (b < b_hi) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int id2 = kv4_page_id(a, en.seq, b + 2 * STEP, b_hi);
+      if (id1 >= 0) load(raw[1 - u], id1, b + STEP);
+      step(raw[u], b, id0 >= 0);
+      b += STEP; id0 = id1; id1 = id2;
+    }
+  }
+  // rows 0 .. RPT - 1 of the sums are in quarter(s) 0 (and 1), as this lane's heads there
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    float t = row_group_sum<16>(l[r]);
+    u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false));
+    t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false)); t = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
+    l[r] = t;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      t = row_group_sum<16>(lov[g][r]);
+      w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false));
+      t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+      if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false)); t = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
+      const float add = fmaf(-128.f, ones[g][r], t);
+#pragma unroll
+      for (int c = 0; c < 4; c++) o[4 * g + c][r] += add;
+    }
+  }
+  const int nv = a.group;
+  if (q4 < RPT / 4) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int c = 4 * q4 + r;
+      if (c < nv) {
+        if (n16 == 0) { s_ml[wv][c][0] = m[r]; s_ml[wv][c][1] = l[r]; }
+#pragma unroll
+        for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + n16] = o[x][r];
+      }
+    }
+  }
+  __syncthreads();
+  kv4_meet<HD, KW>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
 }
 
 // The splits' records of a row (token, query head): a workgroup a row.

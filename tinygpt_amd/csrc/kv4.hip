@@ -19,12 +19,10 @@ int op_err(int code, const char* fmt, ...) {
 struct OnDevice {
   int before = -1, rc = TGX_OK;
   explicit OnDevice(int device) {
-    int n = 0;
+    int cur = -1, n = 0;
+    if (hipGetDevice(&cur) == hipSuccess && cur == device) return;
     if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "no HIP device visible"); return; }
     if (device < 0 || device >= n) { rc = op_err(TGX_ERR_INVALID, "device ordinal %d out of range [0,%d)", device, n); return; }
-    int cur = 0;
-    if (hipGetDevice(&cur) != hipSuccess) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "hipGetDevice failed"); return; }
-    if (cur == device) return;
     if (hipSetDevice(device) != hipSuccess) { (void)hipGetLastError(); rc = op_err(TGX_ERR_DEVICE, "hipSetDevice(%d) failed", device); return; }
     before = cur;
   }
@@ -111,7 +109,9 @@ template <int HD, int TQ, int TP, int TPC>
 static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
   const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries);
   const size_t lds = (size_t)p.kw * std::min<long long>(16, (long long)a.max_count * a.group) * HD * 4;
-  if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  if (a.max_count == 1 && a.group <= 4) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  else if (a.max_count == 1 && a.group <= 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  else if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
   else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, TQ, TP>), grid, dim3(256), lds, s, a);
   else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TPC>), grid, dim3(256), 0, s, a);
 }

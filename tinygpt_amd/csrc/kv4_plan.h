@@ -3,6 +3,7 @@
 #pragma once
 #include <algorithm>
 #include <cstddef>
+#include <cstdlib>
 
 #if defined(__HIPCC__)
 #define TGX_KV4 __host__ __device__ __forceinline__
@@ -93,7 +94,7 @@ inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int
   const long long keys = window > 0 ? std::min<long long>(max_keys, (long long)window + max_count) : max_keys;
   const long long pages = std::max<long long>(1, (keys + KV4_PAGE - 1) / KV4_PAGE);
   const long long wgs = std::max<long long>(1, (long long)entries * kv_heads * p.tiles);
-  const long long want = ((p.kw > 1 ? 4ll : 1ll) * num_cus + wgs - 1) / wgs;
+  const long long want = ((p.kw > 1 ? (getenv("KV4W") ? atoll(getenv("KV4W")) : 2ll) : 1ll) * num_cus + wgs - 1) / wgs;
   p.splits = (int)std::max<long long>(1, std::min<long long>({want, pages, 256}));
   return p;
 }

@@ -10,13 +10,58 @@ the call runs.  Tensors need no particular strides, only a head's channels lie t
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
+import threading
 
 import torch
 
-from .ffi import Kv4BatchArg, Kv4CacheArg, Kv4RowsArg, TgxError, product_backend
+from .ffi import TgxError, product_backend
 
 PAGE_TOKENS = 128
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+# A call's structs (include/tgx.h) are packed into one buffer of the calling thread, at fixed places, and go to the library as addresses: a few calls of a step are short
+# enough for their binding to count (an attention call: 22 us with a ctypes object a struct, 11 so, of which the library and its two launches take most).
+_CACHE, _BATCH, _ROWS = struct.Struct("QqQ5i4x"), struct.Struct("2iq3Q"), struct.Struct("Qi4x2q")
+_AT_CACHE, _AT_BATCH, _AT_Q, _AT_K, _AT_V, _AT_OUT = 0, 64, 128, 160, 192, 224
+_local = threading.local()
+
+
+class _Calls:
+    """the library's entry points, addresses as integers"""
+
+    def __init__(self):
+        self.be = product_backend()
+        p, i, q, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+        for name, res, args in (("kv4_append", i, [p] * 4 + [i, p]), ("kv4_read", i, [p] * 4 + [i, p]), ("kv4_attend_workspace", q, [p, p, i, i, q, i]),
+                                ("kv4_attend", i, [p, p, p, i, p, p, f, i, q, p, p, q, i, p]), ("copy_pages", i, [p, q, q, p, q, q, i, q, p, p, i, i, p])):
+            setattr(self, name, ctypes.CFUNCTYPE(res, *args)(ctypes.cast(getattr(self.be.lib, "tgx_" + name), ctypes.c_void_p).value))
+
+    def check(self, status):
+        if status:
+            raise TgxError(status, (self.be.op_last_error() or b"").decode())
+
+
+@functools.lru_cache(maxsize=None)
+def _calls() -> _Calls:
+    return _Calls()
+
+
+def _buffer():
+    try:
+        return _local.buf, _local.at
+    except AttributeError:
+        _local.buf = ctypes.create_string_buffer(256)
+        _local.at = ctypes.addressof(_local.buf)
+        return _local.buf, _local.at
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(entries, max_count, tokens, kv_heads, head_dim, heads, window, max_keys, device):
+    """bytes of an attention call's workspace: a function of sizes"""
+    cache, batch = _CACHE.pack(16, 1, 16, 1, 1, 1, kv_heads, head_dim), _BATCH.pack(entries, max_count, tokens, 0, 16, 0 if tokens == entries and max_count == 1 else 16)
+    return max(0, _calls().kv4_attend_workspace(ctypes.cast(cache, ctypes.c_void_p), ctypes.cast(batch, ctypes.c_void_p), heads, window, max_keys, device))
 
 
 def kv4_page_bytes(kv_heads: int, head_dim: int) -> int:
@@ -35,23 +80,21 @@ class Kv4Cache:
     does not matter."""
 
     def __init__(self, pool: torch.Tensor, table: torch.Tensor, kv_heads: int, head_dim: int):
-        nbytes = kv_heads * head_dim * 144
         if head_dim not in (64, 128) or kv_heads < 1:
             raise ValueError(f"a 4-bit cache of {kv_heads} heads of {head_dim} channels is not built (head_dim 64 and 128 are)")
-        if pool.dim() < 3 or not pool.is_contiguous() or pool[0, 0].numel() * pool.element_size() != nbytes if pool.numel() else pool.dim() < 3:
+        nbytes, shape = kv_heads * head_dim * 144, pool.shape
+        if len(shape) < 3 or not pool.is_contiguous() or shape[2:].numel() * pool.element_size() != nbytes:
             raise ValueError(f"pool: contiguous [layers][pages][...] with {nbytes} bytes a page")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 and table.shape[1] > 1:
-            raise ValueError("table: int32 [sequences][pages of one], a sequence's entries together")
+        if table.dtype != torch.int32 or table.dim() != 2:
+            raise ValueError("table: int32 [sequences][pages of one]")
+        (seqs, length), (stride, one) = table.shape, table.stride()
+        if length > 1 and one != 1 or seqs > 1 and stride < length:
+            raise ValueError("table: a sequence's entries lie together and are its own")
         if not pool.is_cuda or pool.device != table.device:
             raise ValueError(f"pool ({pool.device}) and table ({table.device}) are on one GPU")
-        self.pool, self.table, self.kv_heads, self.head_dim = pool, table, kv_heads, head_dim
-        self.device = pool.device
-        self._rows_of = {kv_heads: (kv_heads, head_dim)}
-        self._layer_bytes = pool.shape[1] * nbytes
-        stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-        if stride < table.shape[1]:
-            raise ValueError("table: a sequence's entries are its own")
-        self._arg = Kv4CacheArg(pool.data_ptr(), pool.shape[1], table.data_ptr(), stride, table.shape[1], table.shape[0], kv_heads, head_dim)
+        self.pool, self.table, self.kv_heads, self.head_dim, self.device, self.layers = pool, table, kv_heads, head_dim, pool.device, shape[0]
+        self._at, self._layer_bytes = pool.data_ptr(), shape[1] * nbytes
+        self._rest = (shape[1], table.data_ptr(), stride if seqs > 1 else length, length, seqs, kv_heads, head_dim)
 
     @classmethod
     def empty(cls, layers: int, pages: int, kv_heads: int, head_dim: int, seqs: int, max_tokens: int, device="cuda"):
@@ -59,50 +102,48 @@ class Kv4Cache:
         pool = torch.empty(layers, pages, kv4_page_bytes(kv_heads, head_dim), dtype=torch.uint8, device=device)
         return cls(pool, torch.full((seqs, -(-max_tokens // PAGE_TOKENS)), -1, dtype=torch.int32, device=device), kv_heads, head_dim)
 
-    def _at(self, layer: int) -> Kv4CacheArg:
-        if not 0 <= layer < self.pool.shape[0]:
-            raise ValueError(f"layer {layer} of {self.pool.shape[0]}")
-        self._arg.pool = self.pool.data_ptr() + layer * self._layer_bytes
-        return self._arg
+    def _pack(self, buf, layer):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        _CACHE.pack_into(buf, _AT_CACHE, self._at + layer * self._layer_bytes, *self._rest)
 
 
 def _int32(name, t, n, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.stride(0) != 1 and n > 1 or t.device != device:
+    if t.dtype != torch.int32 or t.shape != (n,) or n > 1 and t.stride(0) != 1 or t.device != device:
         raise ValueError(f"{name}: int32 [{n}] without gaps on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _batch(cache, tokens, start, seq, offsets, max_count):
-    entries, dev = start.shape[0], cache.device
+def _pack_batch(buf, cache, tokens, start, seq, offsets, max_count):
+    """(entries, max_count)"""
+    entries, dev = len(start) if start.dim() == 1 else -1, cache.device
     if offsets is None:
         if tokens != entries:
             raise ValueError(f"{tokens} tokens of {entries} entries without offsets (an entry brings one)")
         max_count = 1
     elif max_count is None:
         max_count = tokens
-    return Kv4BatchArg(entries, max_count, tokens, None if seq is None else _int32("seq", seq, entries, dev), _int32("start", start, entries, dev),
-                       None if offsets is None else _int32("offsets", offsets, entries + 1, dev))
+    _BATCH.pack_into(buf, _AT_BATCH, entries, max_count, tokens, 0 if seq is None else _int32("seq", seq, entries, dev), _int32("start", start, entries, dev),
+                     0 if offsets is None else _int32("offsets", offsets, entries + 1, dev))
+    return entries, max_count
 
 
-def _rows(name, t, heads, cache):
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.head_dim:
-        raise ValueError(f"{name}: [tokens][{heads}][{cache.head_dim}], got {tuple(t.shape)}")
-    if t.dtype not in _DTYPES:
+def _pack_rows(buf, at, name, t, tokens, heads, cache):
+    if t.shape != (tokens, heads, cache.head_dim):
+        raise ValueError(f"{name}: [{tokens}][{heads}][{cache.head_dim}], got {tuple(t.shape)}")
+    dtype = _DTYPES.get(t.dtype)
+    if dtype is None:
         raise ValueError(f"{name}: bfloat16, float16 or float32, got {t.dtype}")
     if t.device != cache.device:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.stride(2) != 1:
+    token, head, channel = t.stride()
+    if channel != 1:
         raise ValueError(f"{name}: a head's channels lie together (stride 1)")
-    return Kv4RowsArg(t.data_ptr(), _DTYPES[t.dtype], t.stride(0), t.stride(1))
+    _ROWS.pack_into(buf, at, t.data_ptr(), dtype, token, head)
 
 
-def _check(be, status):
-    if status:
-        raise TgxError(status, (be.op_last_error() or b"").decode())
-
-
-def _where(device):
-    return device.index, torch.cuda.current_stream(device).cuda_stream
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, layer: int = 0, seq: torch.Tensor = None, offsets: torch.Tensor = None,
@@ -111,24 +152,26 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
 
     Entry e brings tokens offsets[e] .. offsets[e + 1] - 1 (int32 [entries + 1]; None: the one token e) of sequence seq[e] (None: e), at positions start[e], start[e] +
     1, ...  max_count: the most that an entry brings (None: all tokens; a smaller grid where it is given).  Positions behind the table's pages are left out."""
-    be = product_backend()
-    b = _batch(cache, k.shape[0], start, seq, offsets, max_count)
-    ka, va = _rows("k", k, cache.kv_heads, cache), _rows("v", v, cache.kv_heads, cache)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError(f"{k.shape[0]} keys and {v.shape[0]} values")
-    _check(be, be.kv4_append(cache._at(layer), b, ka, va, *_where(cache.device)))
+    c, (buf, at) = _calls(), _buffer()
+    tokens = len(k)
+    _pack_batch(buf, cache, tokens, start, seq, offsets, max_count)
+    _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
+    _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
+    cache._pack(buf, layer)
+    c.check(c.kv4_append(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.device.index, _stream(cache.device)))
 
 
 def kv4_read(cache: Kv4Cache, start: torch.Tensor, tokens: int, dtype: torch.dtype = torch.float32, layer: int = 0, seq: torch.Tensor = None, offsets: torch.Tensor = None,
              max_count: int = None, out=None):
     """The values that the cache holds for a batch's tokens, named as in kv4_append: (keys, values), each [tokens][kv_heads][head_dim], rounded once to dtype.
-    out: tensors to write to; tokens that no entry names stay as they were in them."""
-    be = product_backend()
-    k, v = out if out is not None else torch.empty(2, tokens, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device)
-    if k.shape[0] != tokens or v.shape[0] != tokens:
-        raise ValueError(f"out: {tokens} tokens each")
-    b = _batch(cache, tokens, start, seq, offsets, max_count)
-    _check(be, be.kv4_read(cache._at(layer), b, _rows("k", k, cache.kv_heads, cache), _rows("v", v, cache.kv_heads, cache), *_where(cache.device)))
+    out: tensors to write to; tokens that no entry names stay as they were in them (in new ones they hold anything)."""
+    c, (buf, at) = _calls(), _buffer()
+    k, v = out if out is not None else torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device).unbind(0)
+    _pack_batch(buf, cache, tokens, start, seq, offsets, max_count)
+    _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
+    _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
+    cache._pack(buf, layer)
+    c.check(c.kv4_read(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.device.index, _stream(cache.device)))
     return k, v
 
 
@@ -138,29 +181,30 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
 
     The batch's tokens are named as in kv4_append; a token at position p sees its sequence's keys at 0 .. p, with window > 0 the last `window` of them.  k, v: the tokens'
     own keys and values, which join the cache first (then a token sees itself); without them they are there already.  max_keys: at least the last position + 1 of every
-    entry, to divide the work by.  scale: head_dim ** -0.5 where not given.  A token that sees nothing gets zeros."""
-    be = product_backend()
-    heads = q.shape[1] if q.dim() == 3 else 0
-    b = _batch(cache, q.shape[0], start, seq, offsets, max_count)
-    qa = _rows("q", q, heads, cache)
+    entry, to divide the work by.  scale: head_dim ** -0.5 where not given.  A token that sees nothing gets zeros; one that no entry names stays as it was in `out` (in a
+    new one it holds anything)."""
+    c, (buf, at) = _calls(), _buffer()
+    if q.dim() != 3:
+        raise ValueError(f"q: [tokens][heads][{cache.head_dim}], got {tuple(q.shape)}")
+    tokens, heads, _ = q.shape
+    entries, max_count = _pack_batch(buf, cache, tokens, start, seq, offsets, max_count)
+    _pack_rows(buf, _AT_Q, "q", q, tokens, heads, cache)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out: as q")
-    oa = _rows("out", out, heads, cache)
-    ka = va = None
+        out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=cache.device)
+    elif out.dtype != q.dtype:
+        raise ValueError(f"out: {q.dtype} as q, got {out.dtype}")
+    _pack_rows(buf, _AT_OUT, "out", out, tokens, heads, cache)
     if (k is None) != (v is None):
         raise ValueError("k and v come together")
     if k is not None:
-        if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0]:
-            raise ValueError(f"{q.shape[0]} queries, {k.shape[0]} keys and {v.shape[0]} values")
-        ka, va = _rows("k", k, cache.kv_heads, cache), _rows("v", v, cache.kv_heads, cache)
-    c = cache._at(layer)
-    device, stream = _where(cache.device)
-    need = be.kv4_attend_workspace(c, b, heads, window, max_keys, device)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    _check(be, be.kv4_attend(c, b, qa, heads, ka, va, cache.head_dim ** -0.5 if scale is None else scale, window, max_keys, oa, None if ws is None else ws.data_ptr(), max(need, 0),
-                             device, stream))
+        _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
+        _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
+    cache._pack(buf, layer)
+    index = cache.device.index
+    need = _workspace(entries, max_count, tokens, cache.kv_heads, cache.head_dim, heads, window, max_keys, index)
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    c.check(c.kv4_attend(at + _AT_CACHE, at + _AT_BATCH, at + _AT_Q, heads, None if k is None else at + _AT_K, None if k is None else at + _AT_V, cache.head_dim ** -0.5 if scale is None else scale,
+                         window, max_keys, at + _AT_OUT, ws.data_ptr() if need else None, need, index, _stream(cache.device)))
     return out
 
 
@@ -169,17 +213,18 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, into: t
 
     pool, into: [layers][pages][...] whose pages lie without gaps, a multiple of 16 bytes each; src, dst: int32.  A pair with a page that does not exist is left out;
     a page that is copied from is not copied to in the same call, and none is copied to twice."""
-    into = pool if into is None else into
-    be = product_backend()
+    c = _calls()
+    n = len(src) if src.dim() == 1 else -1
     sizes = []
-    for name, t in (("pool", pool), ("into", into)):
-        if t.dim() < 3 or not t.is_cuda or t.numel() and not t[0].is_contiguous():
+    for name, t in (("pool", pool),) if into is None else (("pool", pool), ("into", into)):
+        shape = t.shape
+        if len(shape) < 3 or not t.is_cuda or not t.is_contiguous() and t.numel() and not t[0].is_contiguous():
             raise ValueError(f"{name}: [layers][pages][...] on a GPU, a layer's pages without gaps")
-        sizes.append(t.shape[2:].numel() * t.element_size())
-    if sizes[0] != sizes[1] or pool.shape[0] != into.shape[0] or pool.device != into.device:
-        raise ValueError(f"pools of {pool.shape[0]} and {into.shape[0]} layers, pages of {sizes[0]} and {sizes[1]} bytes, on {pool.device} and {into.device}")
-    n = src.shape[0] if src.dim() == 1 else -1
-    args = (_int32("src", src, n, pool.device), _int32("dst", dst, n, pool.device), n)
-    _check(be, be.copy_pages(pool.data_ptr(), pool.shape[1], pool.stride(0) * pool.element_size(), into.data_ptr(), into.shape[1], into.stride(0) * into.element_size(),
-                             pool.shape[0], sizes[0], *args, *_where(pool.device)))
-    return into
+        es = t.element_size()
+        sizes.append((t.data_ptr(), shape[1], t.stride(0) * es, shape[0], shape[2:].numel() * es))
+    a, b = sizes[0], sizes[-1]
+    if into is not None and (a[3:] != b[3:] or pool.device != into.device):
+        raise ValueError(f"pools of {a[3]} and {b[3]} layers, pages of {a[4]} and {b[4]} bytes, on {pool.device} and {into.device}")
+    dev = pool.device
+    c.check(c.copy_pages(*a[:3], *b[:3], a[3], a[4], _int32("src", src, n, dev), _int32("dst", dst, n, dev), n, dev.index, _stream(dev)))
+    return pool if into is None else into
