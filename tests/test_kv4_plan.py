@@ -67,8 +67,8 @@ extern "C" int ranges(int first, int last, int window, int len, int splits) {
   const int want = last < 0 ? 0 : (last / 128 + 1 < len ? last / 128 + 1 : len), lo = window > 0 && first - window + 1 > 0 ? (first - window + 1) / 128 : 0;
   return end == (want > lo ? want : 0) ? 0 : 4;
 }
-extern "C" void plan(int entries, int max_count, int kv_heads, int group, int window, long long keys, int cus, int* out) {
-  const Kv4Plan p = kv4_plan(entries, max_count, kv_heads, group, window, keys, cus);
+extern "C" void plan(int entries, int max_count, int kv_heads, int group, int hd, int window, long long keys, int cus, int* out) {
+  const Kv4Plan p = kv4_plan(entries, max_count, kv_heads, group, hd, window, keys, cus);
   out[0] = p.kw; out[1] = p.nt; out[2] = p.tiles; out[3] = p.splits;
 }
 """
@@ -83,7 +83,7 @@ def plan(tmp_path_factory):
     so = ctypes.CDLL(str(lib))
     so.page.restype = ctypes.c_longlong
     so.entry.argtypes = [ctypes.c_int] * 5 + [ctypes.c_longlong, ctypes.c_int]
-    so.plan.argtypes = [ctypes.c_int] * 5 + [ctypes.c_longlong, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+    so.plan.argtypes = [ctypes.c_int] * 6 + [ctypes.c_longlong, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
     return so
 
 
@@ -126,11 +126,13 @@ def test_plans_cover_their_columns(plan, cus):
         for count in [1, 2, 5, 17, 200, 2048, 65535]:
             for group in [1, 4, 7, 16]:
                 for window, keys in [(0, 1), (0, 131072), (64, 131072), (0, 2 ** 31 - 1), (0, 0)]:
-                    plan.plan(entries, count, 8, group, window, keys, cus, out)
-                    kw, nt, tiles, splits = out
-                    assert kw in (1, 4) and tiles * 16 * nt * (1 if kw == 4 else 4) >= count * group and 1 <= splits <= 256
-                    if kw == 4 and nt == 1:
-                        assert tiles == 1      # a single token's keys and values are appended by one workgroup a (entry, head, split)
+                    for hd in (64, 128):
+                        plan.plan(entries, count, 8, group, hd, window, keys, cus, out)
+                        kw, nt, tiles, splits = out
+                        assert kw in (1, 4, 8) and tiles * 16 * nt * (1 if kw > 1 else 4) >= count * group and 1 <= splits <= 256
+                        assert kw < 8 or count == 1 and group <= 8
+                        if kw > 1 and nt == 1:
+                            assert tiles == 1      # a single token's keys and values are appended by one workgroup a (entry, head, split)
 
 
 # ---- what is refused, before a GPU is touched ---------------------------------------------------------------------------------------------------------

@@ -30,11 +30,6 @@ __device__ __forceinline__ float kv4_load(const void* p, long long i, int dt) {
   const unsigned short u = static_cast<const unsigned short*>(p)[i];
   return dt == DT_BF16 ? bf16_to_f32(u) : f16_bits_to_f32(u);
 }
-__device__ __forceinline__ void kv4_store(void* p, long long i, float v, int dt) {
-  if (dt == DT_F32) static_cast<float*>(p)[i] = v;
-  else static_cast<unsigned short*>(p)[i] = dt == DT_BF16 ? f32_to_bf16(v) : f32_to_f16_bits(v);
-}
-
 // ---- one group's levels ----------------------------------------------------------------------------------------------------------------------------
 struct Kv4Levels { float lo, inv; unsigned int word; };       // word: the group's parameter word
 __device__ __forceinline__ Kv4Levels kv4_levels(float mn, float mx, bool bad) {
@@ -300,47 +295,47 @@ __device__ __forceinline__ int kv4_page_id(const Kv4Args& a, int seq, int b, int
   const int p = *(const __attribute__((address_space(4))) int*)at;
   return p >= 0 && p < a.pages ? p : -1;
 }
-// eight neighbouring channels of a row of a runtime type
-__device__ __forceinline__ void kv4_load8(const void* p, long long i, int dt, float x[8]) {
-  if (dt == DT_F32) {
-    const float* f = static_cast<const float*>(p) + i;
-    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) slice_unpack<DT_F32>(load_slice<DT_F32>(f, 0), x);
-    else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = f[e];
-    }
-    return;
-  }
-  const unsigned short* u = static_cast<const unsigned short*>(p) + i;
-  u32x4 w;
-  if ((reinterpret_cast<uintptr_t>(u) & 15) == 0) w = *reinterpret_cast<const u32x4*>(u);
+// a query's and an output's type by the terms of a query
+template <int TQ> constexpr int kv4_type() { return TQ == 1 ? DT_BF16 : TQ == 2 ? DT_F16 : DT_F32; }
+// eight neighbouring channels of a row
+template <int DT>
+__device__ __forceinline__ void kv4_load8(const void* p, long long i, float x[8]) {
+  const elem_t<DT>* e = static_cast<const elem_t<DT>*>(p) + i;
+  if ((reinterpret_cast<uintptr_t>(e) & 15) == 0) slice_unpack<DT>(load_slice<DT>(e, 0), x);
   else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) w[e] = u[2 * e] | ((unsigned int)u[2 * e + 1] << 16);
+    for (int c = 0; c < 8; c++) x[c] = elem_to_f32<DT>(e[c]);
   }
-  Slice8<DT_BF16> s{w};
-  if (dt == DT_BF16) slice_unpack<DT_BF16>(s, x);
-  else slice_unpack<DT_F16>(Slice8<DT_F16>{w}, x);
 }
-__device__ __forceinline__ void kv4_store4(void* p, long long i, const f32x4 v, int dt) {
-  if (dt == DT_F32) {
-    float* f = static_cast<float*>(p) + i;
-    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) *reinterpret_cast<f32x4*>(f) = v;
+// four neighbouring channels of an output; mode: rounded to a storage type first (32-bit outputs; option act.round16 of a model)
+template <int DT>
+__device__ __forceinline__ void kv4_store4(void* p, long long i, const f32x4 v, int mode) {
+  elem_t<DT>* e = static_cast<elem_t<DT>*>(p) + i;
+  if constexpr (DT == DT_F32) {
+    f32x4 r = v;
+    if (mode) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) r[c] = round_storage_mode(v[c], mode);
+    }
+    if ((reinterpret_cast<uintptr_t>(e) & 15) == 0) *reinterpret_cast<f32x4*>(e) = r;
     else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) f[e] = v[e];
+      for (int c = 0; c < 4; c++) e[c] = r[c];
     }
-    return;
-  }
-  unsigned short* u = static_cast<unsigned short*>(p) + i;
-  unsigned short h[4];
+  } else {
+    elem_t<DT> h[4];
 #pragma unroll
-  for (int e = 0; e < 4; e++) h[e] = dt == DT_BF16 ? f32_to_bf16(v[e]) : f32_to_f16_bits(v[e]);
-  if ((reinterpret_cast<uintptr_t>(u) & 7) == 0) *reinterpret_cast<u32x2*>(u) = u32x2{h[0] | ((unsigned int)h[1] << 16), h[2] | ((unsigned int)h[3] << 16)};
-  else {
+    for (int c = 0; c < 4; c++) h[c] = f32_to_elem<DT>(v[c]);
+    if ((reinterpret_cast<uintptr_t>(e) & 7) == 0) *reinterpret_cast<u32x2*>(e) = u32x2{h[0] | ((unsigned int)h[1] << 16), h[2] | ((unsigned int)h[3] << 16)};
+    else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) u[e] = h[e];
+      for (int c = 0; c < 4; c++) e[c] = h[c];
+    }
   }
+}
+template <int DT>
+__device__ __forceinline__ void kv4_store1(void* p, long long i, float v, int mode) {
+  static_cast<elem_t<DT>*>(p)[i] = f32_to_elem<DT>(DT == DT_F32 && mode ? round_storage_mode(v, mode) : v);
 }
 
 // a block's codes and parameters on their way: key and value words as operands, the parameters of token (lane & 31)
@@ -382,7 +377,7 @@ struct Kv4Sums {
 #pragma unroll
       for (int ch = 0; ch < CH; ch++) {
         float x[8];
-        kv4_load8(a.q, base + 32 * ch, a.q_dt, x);
+        kv4_load8<kv4_type<TQ>()>(a.q, base + 32 * ch, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
 #pragma unroll
@@ -579,7 +574,7 @@ struct Kv4Sums {
 };
 
 // The waves' sums of up to 16 columns meet in LDS: so [KW][columns][HD], a thread takes four channels of a column through all waves; the split's record, or the output.
-template <int HD, int KW>
+template <int HD, int KW, int DT>
 __device__ __forceinline__ void kv4_meet(const Kv4Args& a, const Kv4Entry& en, int kvh, int split, int c0, int nv, const float* so, const float (*s_ml)[16][2]) {
   for (int item = threadIdx.x; item < nv * (HD / 4); item += 64 * KW) {
     const int c = item / (HD / 4), x = item % (HD / 4);
@@ -604,8 +599,8 @@ __device__ __forceinline__ void kv4_meet(const Kv4Args& a, const Kv4Entry& en, i
     } else {
       const float inv = den == 0.f ? 0.f : 1.f / den;      // a row that sees nothing gives zeros
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[e] = round_storage_mode(acc[e] * inv, a.act16);
-      kv4_store4(a.out, (en.tok0 + i) * a.o_ts + h * a.o_hs + 4 * x, acc, a.q_dt);
+      for (int e = 0; e < 4; e++) acc[e] *= inv;
+      kv4_store4<DT>(a.out, (en.tok0 + i) * a.o_ts + h * a.o_hs + 4 * x, acc, a.act16);
     }
   }
 }
@@ -661,7 +656,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
         for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + r16] = s.o[t][x][r];
     }
     __syncthreads();
-    kv4_meet<HD, KW>(a, en, kvh, split, c0, nv, kv4_lds, s_ml);
+    kv4_meet<HD, KW, kv4_type<TQ>()>(a, en, kvh, split, c0, nv, kv4_lds, s_ml);
   }
 }
 
@@ -708,7 +703,7 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
         const float inv = den == 0.f ? 0.f : 1.f / den;
         const long long at = (en.tok0 + i) * a.o_ts + h * a.o_hs;
 #pragma unroll
-        for (int x = 0; x < CT; x++) kv4_store(a.out, at + 16 * x + r16, round_storage_mode(s.o[t][x][r] * inv, a.act16), a.q_dt);
+        for (int x = 0; x < CT; x++) kv4_store1<kv4_type<TQ>()>(a.out, at + 16 * x + r16, s.o[t][x][r] * inv, a.act16);
       }
     }
   }
@@ -739,27 +734,30 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5) & ~(NB - 1);      // (a step's blocks are of one page)
   const int tile = RPT == 4 ? q4 : q4 >> 1;                       // this lane's token of a step: 16 tile + n16, heads h0 .. h0 + 3
   const int h0 = RPT == 4 ? 0 : 4 * (q4 & 1);
-  struct Raw { u32x4 k[NB][PARTS], v[NB][PARTS]; unsigned int p[PW]; };
+  u32x4 rk[NB][PARTS] = {}, rv[NB][PARTS] = {};                   // a step's codes (of no block: numbers too) and its token's parameters
+  unsigned int rp[PW] = {};
   const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
   const size_t page_words = (size_t)a.kv_heads * (36 * HD);
-  auto load = [&](Raw& raw, int id, int b) {
+  auto load_keys = [&](int id, int b) {
     const unsigned int* blk = heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>();
 #pragma unroll
     for (int x = 0; x < NB; x++)
 #pragma unroll
-      for (int i = 0; i < PARTS; i++) raw.k[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>()) + i * 64 + lane);
+      for (int i = 0; i < PARTS; i++) rk[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>()) + i * 64 + lane);
     const unsigned int* pw = blk + (tile >> 1) * kv4_block_words<HD>() + 8 * HD + (16 * (tile & 1) + n16) * PW;
-    if constexpr (PW == 4) { const u32x4 w = load_nt(reinterpret_cast<const u32x4*>(pw)); raw.p[0] = w[0]; raw.p[1] = w[1]; raw.p[2] = w[2]; raw.p[3] = w[3]; }
-    else { const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(pw)); raw.p[0] = w[0]; raw.p[1] = w[1]; }
+    if constexpr (PW == 4) { const u32x4 w = load_nt(reinterpret_cast<const u32x4*>(pw)); rp[0] = w[0]; rp[1] = w[1]; rp[2] = w[2]; rp[3] = w[3]; }
+    else { const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(pw)); rp[0] = w[0]; rp[1] = w[1]; }
+  };
+  auto load_values = [&](int id, int b) {
+    const unsigned int* blk = heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>() + 4 * HD;
 #pragma unroll
     for (int x = 0; x < NB; x++)
 #pragma unroll
-      for (int i = 0; i < PARTS; i++) raw.v[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>() + 4 * HD) + i * 64 + lane);
+      for (int i = 0; i < PARTS; i++) rv[x][i] = load_nt(reinterpret_cast<const u32x4*>(blk + x * kv4_block_words<HD>()) + i * 64 + lane);
   };
   constexpr int STEP = KW * NB;
-  Raw raw[2] = {};                                                // (codes of no block are numbers too)
   int b = b_lo + wv * NB, id0 = kv4_page_id(a, en.seq, b, b_hi), id1 = kv4_page_id(a, en.seq, b + STEP, b_hi);
-  if (id0 >= 0) load(raw[0], id0, b);
+  if (id0 >= 0) { load_keys(id0, b); load_values(id0, b); }
   // queries: row n16 = head n16 % RPT, channels 32 c + 8 q .. + 7; the sums of a group's channels per head of this lane
   bf16x8_t qf[CH][TQ];
   float qs[G][4];
@@ -771,7 +769,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 #pragma unroll
     for (int ch = 0; ch < CH; ch++) {
       float x[8];
-      kv4_load8(a.q, base + 32 * ch, a.q_dt, x);
+      kv4_load8<kv4_type<TQ>()>(a.q, base + 32 * ch, x);
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
 #pragma unroll
@@ -809,14 +807,16 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   const int w_at = (tile >> 1) * 32 + (n16 >> 2) * 8 + (n16 & 3) + 4 * (tile & 1);      // this lane's token among a head's weights
   const float scale = a.scale_log2, gap = a.gap;
 
-  // one step: NB blocks from block bb on; what is not seen (or there) has levels of zero and a score of -inf
-  auto step = [&](const Raw& rw, int bb, bool there) {
-    const int j = bb * KV4_BLK + 16 * tile + n16;
-    const bool in = there && j >= key_lo && j <= last;
+  // Steps: NB blocks each; what is not seen (or there) has levels of zero and a score of -inf.  The next step's keys are asked for when this one's are products, its values behind
+  // P V, the page of the step behind in front of both: one set of registers, and no branch around the sums.
+  for (; b < b_hi; b += STEP) {
+    const int id2 = kv4_page_id(a, en.seq, b + 2 * STEP, b_hi);
+    const int j = b * KV4_BLK + 16 * tile + n16;
+    const bool in = id0 >= 0 && j >= key_lo && j <= last;
     float st[2][G], lo[2][G];
 #pragma unroll
     for (int w = 0; w < PW; w++) {
-      const unsigned int x = in ? rw.p[w] : 0u;
+      const unsigned int x = in ? rp[w] : 0u;
       st[w / G][w % G] = bf16_hi(x); lo[w / G][w % G] = bf16_lo(x);
     }
     const float begin = in ? 0.f : -INFINITY;
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           const int x = (t & 1) * CH + 2 * g + c;
-          const bf16x8_t kf = kv4_frag(rw.k[t >> 1][x >> 2][x & 3], mask, off);
+          const bf16x8_t kf = kv4_frag(rk[t >> 1][x >> 2][x & 3], mask, off);
 #pragma unroll
           for (int term = 0; term < TQ; term++) d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[2 * g + c][term], kf, d[t], 0, 0, 0);
         }
@@ -845,6 +845,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (id1 >= 0) load_keys(id1, b + STEP);
     if (__any(sc[0] > m[0] + gap || sc[1] > m[1] + gap || sc[2] > m[2] + gap || sc[3] > m[3] + gap)) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -901,26 +902,22 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
       for (int x = 0; x < NB; x++) {
 #pragma unroll
         for (int term = 0; term < TP; term++) ones[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], one8, ones[g], 0, 0, 0);
+        bf16x8_t vf[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           const int i = 4 * g + c;
-          const bf16x8_t vf = kv4_frag(rw.v[x][i >> 2][i & 3], mask, off);
-#pragma unroll
-          for (int term = 0; term < TP; term++) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], vf, o[i], 0, 0, 0);
+          vf[c] = kv4_frag(rv[x][i >> 2][i & 3], mask, off);
+          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][0], vf[c], o[i], 0, 0, 0);
         }
+#pragma unroll
+        for (int term = 1; term < TP; term++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[4 * g + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], vf[c], o[4 * g + c], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-  };
-  // one step on its way while one is worked on, the page of the one behind on its way before that; no branch but the loop's around the sums
-  while (b < b_hi) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int id2 = kv4_page_id(a, en.seq, b + 2 * STEP, b_hi);
-      if (id1 >= 0) load(raw[1 - u], id1, b + STEP);
-      step(raw[u], b, id0 >= 0);
-      b += STEP; id0 = id1; id1 = id2;
-    }
+    if (id1 >= 0) load_values(id1, b + STEP);
+    id0 = id1; id1 = id2;
   }
   // rows 0 .. RPT - 1 of the sums are in quarter(s) 0 (and 1), as this lane's heads there
 #pragma unroll
@@ -954,11 +951,11 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
     }
   }
   __syncthreads();
-  kv4_meet<HD, KW>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
+  kv4_meet<HD, KW, kv4_type<TQ>()>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
 }
 
 // The splits' records of a row (token, query head): a workgroup a row.
-template <int HD>
+template <int HD, int DT>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
   constexpr int LN = HD / 4, WAYS = 256 / LN;                 // lanes of a row, splits at a time
   __shared__ float sw[1024];
@@ -1002,8 +999,8 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
     const float inv = stot == 0.f ? 0.f : 1.f / stot;
     const long long at = (en.tok0 + blockIdx.y) * a.o_ts + h * a.o_hs + 4 * tid;
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = round_storage_mode(acc[i] * inv, a.act16);
-    kv4_store4(a.out, at, acc, a.q_dt);
+    for (int i = 0; i < 4; i++) acc[i] *= inv;
+    kv4_store4<DT>(a.out, at, acc, a.act16);
   }
 }
 

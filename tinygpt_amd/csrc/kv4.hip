@@ -109,8 +109,13 @@ template <int HD, int TQ, int TP, int TPC>
 static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
   const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries);
   const size_t lds = (size_t)p.kw * std::min<long long>(16, (long long)a.max_count * a.group) * HD * 4;
-  if (a.max_count == 1 && a.group <= 4) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 4, TQ, TP>), grid, dim3(256), lds, s, a);
-  else if (a.max_count == 1 && a.group <= 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  if (a.max_count == 1 && a.group <= 4) {
+    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 8, TQ, TP>), grid, dim3(512), lds, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  } else if (a.max_count == 1 && a.group <= 8) {
+    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 8, TQ, TP>), grid, dim3(512), lds, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+  }
   else if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
   else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, TQ, TP>), grid, dim3(256), lds, s, a);
   else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TPC>), grid, dim3(256), 0, s, a);
@@ -135,8 +140,9 @@ void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws,
   }
   if (p.splits > 1) {
     const dim3 grid(a.heads, a.max_count, a.entries);
-    if (hd == 64) hipLaunchKernelGGL(tgx::kv4_combine_kernel<64>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(tgx::kv4_combine_kernel<128>, grid, dim3(256), 0, s, a);
+    TGX_DT_SWITCH(a.q_dt,
+      if (hd == 64) hipLaunchKernelGGL((tgx::kv4_combine_kernel<64, DT>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((tgx::kv4_combine_kernel<128, DT>), grid, dim3(256), 0, s, a);)
   }
 }
 
@@ -199,7 +205,7 @@ int64_t tgx_kv4_attend_workspace(const tgx_kv4_cache* cache, const tgx_kv4_batch
   tgx::Kv4Args a{};
   if (attend_args(cache, batch, heads, window, max_keys, a)) return -1;
   if (!a.entries || !a.max_count || !a.tokens) return 0;
-  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, window, max_keys, num_cus_of(device));
+  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, cache->head_dim, window, max_keys, num_cus_of(device));
   return (int64_t)tgx::kv4_part_floats(p, a.tokens * heads, cache->head_dim) * 4;
 }
 
@@ -219,7 +225,7 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   if (!a.max_count || !a.tokens) return TGX_OK;
   OnDevice on(device);
   if (on.rc) return on.rc;
-  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, window, max_keys, num_cus_of(device));
+  const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, cache->head_dim, window, max_keys, num_cus_of(device));
   const int64_t need = (int64_t)tgx::kv4_part_floats(p, a.tokens * heads, cache->head_dim) * 4;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return op_err(TGX_ERR_INVALID, "workspace: %lld bytes aligned to 16 are needed", (long long)need);
   if (p.tiles > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);

@@ -3,7 +3,6 @@
 #pragma once
 #include <algorithm>
 #include <cstddef>
-#include <cstdlib>
 
 #if defined(__HIPCC__)
 #define TGX_KV4 __host__ __device__ __forceinline__
@@ -82,20 +81,29 @@ TGX_KV4 Kv4Range kv4_range(int first, int last, int window, int table_len, int s
 }
 
 // How a batch's attention is divided: kw > 1 = the kw waves of a workgroup share nt * 16 columns (token, query head) and divide the keys, kw 1 = four waves divide the columns;
-// tiles workgroups of columns, splits of the keys between workgroups
+// tiles workgroups of columns, splits of the keys between workgroups (their records meet in a launch of their own)
 struct Kv4Plan { int kw, nt, tiles, splits; };
-inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int window, long long max_keys, int num_cus) {
+inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int hd, int window, long long max_keys, int num_cus) {
   Kv4Plan p;
   const long long cols = (long long)max_count * group;
   p.kw = cols <= 32 ? 4 : 1;
-  p.nt = p.kw > 1 ? (cols <= 16 ? 1 : 2) : 2;
+  p.nt = p.kw > 1 && cols <= 16 ? 1 : 2;
   const int per = 16 * p.nt * (p.kw > 1 ? 1 : 4);
   p.tiles = (int)((cols + per - 1) / per);
   const long long keys = window > 0 ? std::min<long long>(max_keys, (long long)window + max_count) : max_keys;
   const long long pages = std::max<long long>(1, (keys + KV4_PAGE - 1) / KV4_PAGE);
   const long long wgs = std::max<long long>(1, (long long)entries * kv_heads * p.tiles);
-  const long long want = ((p.kw > 1 ? (getenv("KV4W") ? atoll(getenv("KV4W")) : 2ll) : 1ll) * num_cus + wgs - 1) / wgs;
+  // Two workgroups a compute unit where the waves divide the keys, one where they divide the columns: with more, a wave walks fewer blocks behind the same way in and out.  us, one / two / three / four
+  // workgroups a compute unit, four waves each: 32 rows of up to 4096 tokens, head_dim 128, 33.3 / 24.7 / 30.0 / 32.5; one of 131071 45.1 / 33.8 / 33.4 / 39.1; 64 of 1500, head_dim 64,
+  // 11.7 / 8.9 / 10.4 / 11.8.
+  const long long want = ((p.kw > 1 ? 2ll : 1ll) * num_cus + wgs - 1) / wgs;
   p.splits = (int)std::max<long long>(1, std::min<long long>({want, pages, 256}));
+  // The records' launch and the way to it cost 3.3 us; a page of 128 tokens walked by one workgroup 0.29 us at head_dim 64, 0.5 at 128 (eight waves).  us whole / split, eight heads of one row: head_dim 64,
+  // 700 tokens 6.3 / 8.1, 1024 7.1 / 8.1, 1500 8.6 / 8.1; head_dim 128, 512 8.1 / 9.1, 700 8.8 / 9.2, 1024 10.5 / 9.3; 16 rows of head_dim 128, 1024 11.3 / 12.7, 2048 16.3 / 15.5.
+  if (p.kw > 1 && pages * (p.splits - 1) * (hd / 64) <= 12ll * p.splits) p.splits = 1;
+  // A single token's keys whole in a workgroup: eight waves where there is a compute unit for each workgroup (16 rows of head_dim 128, 2048 tokens, four waves / eight: 17.4 / 16.3;
+  // one row of head_dim 64, 1024: 7.4 / 7.1) or the walk is long (64 rows of eight heads, head_dim 64: 1024 tokens 11.5 / 12.7, 3000 24.9 / 23.0)
+  if (max_count == 1 && group <= 8 && p.splits == 1 && (wgs <= num_cus ? pages > 2 : pages >= 16)) p.kw = 8;
   return p;
 }
 inline size_t kv4_part_floats(const Kv4Plan& p, long long rows, int hd) { return p.splits > 1 ? (size_t)rows * p.splits * (hd + 2) : 0; }      // workspace of the splits' records
