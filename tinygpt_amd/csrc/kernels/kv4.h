@@ -12,7 +12,7 @@
 // nothing passes through LDS: word (part * 64 + lane) * 4 + w, lane = 16 q + r, i = 4 part + w,
 //   keys    token 16 (i / (HD / 32)) + r, channels 32 (i % (HD / 32)) + 8 q + e        (the A operand of a 16 x 16 x 32 product: rows tokens)
 //   values  channel 16 i + r, token 4 q + e (e < 4) or 16 + 4 q + e - 4                 (the B operand, its contraction in the order in which the scores' lanes hold the tokens)
-// e = 0 .. 7 at bit 4 (e / 2 + 4 (e % 2)): (w >> 4 i) & 0x000f000f | 0x43004300 is the pair (2 i, 2 i + 1) as bf16 128 + n, exactly.
+// e = 0 .. 7 at bit 4 (e / 2 + 4 (e % 2)).
 // Parameters: [32 tokens][keys, values][HD / 64] words, lo in the low half, step in the high.
 #pragma once
 #include "common.h"
@@ -261,20 +261,25 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------------------------------------------
-// S^T = K Q^T with the codes as the operand: a score is sum_g step_g (q_g . (128 + n_g)) + (lo_g - 128 step_g) sum(q_g), so that a product of 16 tokens x 16 query
-// columns (column = token of the entry, query head of the kv head) costs two fused multiply-adds a score and group and no value is unpacked.  O = P V the same
-// way: the weights p step_g (bf16, TP terms of them) meet 128 + n; what the 128 adds is taken off with the weights' own sum (a product with ones: the same rounded
-// weights), the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A operand
-// of P V, whose contraction runs over the tokens in the order of the value words.
+// S^T = K Q^T with the codes as the operand: a score is sum_g step_g (q_g . n_g) + lo_g sum(q_g), so that a product of 16 tokens x 16 query columns (column = token of the
+// entry, query head of the kv head) costs two fused multiply-adds a score and group and no value is worked out.  O = P V the same way: the weights p step_g (bf16, TP terms of
+// them) meet the codes, the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A
+// operand of P V, whose contraction runs over the tokens in the order of the value words.
 // TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17) leave an output
-// in 16 bits what its own rounding leaves, three one in 32.  One term (2^-9, as coarse as an output in bf16) is taken off the levels' middle: 136 in the place of 128
-// and lo + 8 step in the place of lo, so that its rounding meets numbers as large as the values and not as their spread.
-__device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w, unsigned int mask, unsigned int off) {
+// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, took a portion of 2048 tokens from 672 us to 573 and left it 1.55 times as far from
+// 64 bits: its rounding meets the levels' spread.)
+// A word's codes as bf16 numbers, exactly: a byte n of 0 .. 15 is the fp8 (e4m3) number n / 512, and the conversion scales.  They come in the order e = 0, 4, 1, 5, 2, 6, 3, 7, in which
+// what they are multiplied with is laid out (kv4_slot: the code at a place).
+__device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
+  const unsigned int a = w & 0x0f0f0f0fu, b = (w >> 4) & 0x0f0f0f0fu;
   u32x4 f;
-#pragma unroll
-  for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & mask) | off;
+  f[0] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, false));
+  f[1] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, true));
+  f[2] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, false));
+  f[3] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, true));
   return __builtin_bit_cast(bf16x8_t, f);
 }
+constexpr int kv4_slot[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 // over the lanes of equal r: lanes 16 and 32 further swap in the vector registers
 __device__ __forceinline__ float kv4_max_quarters(float v) {
   u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
@@ -356,11 +361,10 @@ template <int HD> struct Kv4Raw {
 template <int HD, int NT, int TQ, int TP>
 struct Kv4Sums {
   static constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16;
-  static constexpr bool CENTRE = TP == 1;
   bf16x8_t qf[NT][CH][TQ];
   float qsum[NT][G];
   int pos[NT];                                                // a column's position; -1: no column
-  f32x4 o[NT][CT], ones[NT][G];
+  f32x4 o[NT][CT];
   float m[NT], l[NT], lov[NT][G];                             // m: the reference of the weights, in scores before the scale
 
   __device__ __forceinline__ void start(const Kv4Args& a, const Kv4Entry& en, int kvh, int col0, int ncol, int q4, int r16) {
@@ -371,7 +375,7 @@ struct Kv4Sums {
       const long long base = (en.tok0 + i) * a.q_ts + h * a.q_hs + 8 * q4;
       m[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; g++) { qsum[t][g] = 0.f; lov[t][g] = 0.f; ones[t][g] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+      for (int g = 0; g < G; g++) { qsum[t][g] = 0.f; lov[t][g] = 0.f; }
 #pragma unroll
       for (int x = 0; x < CT; x++) o[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -385,9 +389,9 @@ struct Kv4Sums {
           u32x4 f;
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            f[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+            f[e] = pack_bf16(x[kv4_slot[2 * e]], x[kv4_slot[2 * e + 1]]);
             qsum[t][ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
-            x[2 * e] -= bf16_lo(f[e]); x[2 * e + 1] -= bf16_hi(f[e]);
+            x[kv4_slot[2 * e]] -= bf16_lo(f[e]); x[kv4_slot[2 * e + 1]] -= bf16_hi(f[e]);
           }
           qf[t][ch][term] = __builtin_bit_cast(bf16x8_t, f);
         }
@@ -400,7 +404,7 @@ struct Kv4Sums {
   // One block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters, which every lane needs of the four tokens of its scores.  MASK: some column does not
   // see some token of the block; what is not seen is selected away, whatever it holds.  In phases that the compiler does not mix: mixed, their registers are half again as many.
   template <bool MASK>
-  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, unsigned int* sp, int lane) {
     const int q4 = lane >> 4;
     constexpr int PW = HD / 32;                               // parameter words of a token: keys, then values
     if constexpr (PW == 4) *reinterpret_cast<u32x4*>(sp + (lane & 31) * 4) = u32x4{raw.p[0], raw.p[1], raw.p[2], raw.p[3]};
@@ -425,10 +429,10 @@ struct Kv4Sums {
       for (int g = 0; g < G; g++) {
         bf16x8_t kf[2];
 #pragma unroll
-        for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(raw.k[x >> 2][x & 3], mask, off); }
+        for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(raw.k[x >> 2][x & 3]); }
         float st[4], z[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) { st[r] = bf16_hi(par[i][r][g]); z[r] = fmaf(-128.f, st[r], bf16_lo(par[i][r][g])); }
+        for (int r = 0; r < 4; r++) { st[r] = bf16_hi(par[i][r][g]); z[r] = bf16_lo(par[i][r][g]); }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -468,8 +472,6 @@ struct Kv4Sums {
           const float fr = __shfl(f, 4 * q4 + r, 64);
 #pragma unroll
           for (int c = 0; c < CT; c++) o[t][c][r] *= fr;
-#pragma unroll
-          for (int g = 0; g < G; g++) ones[t][g][r] *= fr;
         }
       }
       const float ref = -m[t] * scale;
@@ -485,7 +487,6 @@ struct Kv4Sums {
     __builtin_amdgcn_sched_barrier(0);
     parameters(par, 1);
     wave_fence();
-    const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
     for (int g = 0; g < G; g++) {
       u32x4 pf[NT][TP];
@@ -497,7 +498,7 @@ struct Kv4Sums {
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const unsigned int w = par[i][r][g];
-            const float st = bf16_hi(w), lo = CENTRE ? fmaf(8.f, st, bf16_lo(w)) : bf16_lo(w);
+            const float st = bf16_hi(w), lo = bf16_lo(w);
             ps[4 * i + r] = MASK && !seen[t][i][r] ? 0.f : p[t][i][r] * st;
             lov[t][g] = MASK && !seen[t][i][r] ? lov[t][g] : fmaf(p[t][i][r], lo, lov[t][g]);
           }
@@ -505,16 +506,14 @@ struct Kv4Sums {
         for (int term = 0; term < TP; term++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            pf[t][term][e] = pack_bf16(ps[2 * e], ps[2 * e + 1]);
-            if (term + 1 < TP) { ps[2 * e] -= bf16_lo(pf[t][term][e]); ps[2 * e + 1] -= bf16_hi(pf[t][term][e]); }
+            pf[t][term][e] = pack_bf16(ps[kv4_slot[2 * e]], ps[kv4_slot[2 * e + 1]]);
+            if (term + 1 < TP) { ps[kv4_slot[2 * e]] -= bf16_lo(pf[t][term][e]); ps[kv4_slot[2 * e + 1]] -= bf16_hi(pf[t][term][e]); }
           }
-#pragma unroll
-        for (int term = 0; term < TP; term++) ones[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][term]), one8, ones[t][g], 0, 0, 0);
       }
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const int x = 4 * g + c;
-        const bf16x8_t vf = kv4_frag(raw.v[x >> 2][x & 3], mask, off);
+        const bf16x8_t vf = kv4_frag(raw.v[x >> 2][x & 3]);
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -527,7 +526,7 @@ struct Kv4Sums {
   // The blocks b0, b0 + STEP, .. below b1, every one (MASK false) or only those of them outside of [skip0, skip1) (MASK true): one on its way while one is worked on, the page of the one behind on its way
   // before that.  A walk takes one kind of block: with both in one loop the compiler keeps two sets of sums.
   template <bool MASK, int STEP>
-  __device__ __forceinline__ void walk(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+  __device__ __forceinline__ void walk(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, unsigned int* sp, int lane) {
     const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
     const size_t page_words = (size_t)a.kv_heads * (36 * HD);
     auto past = [&](int b) { return MASK && b >= skip0 && b < skip1 ? b + (skip1 - b + STEP - 1) / STEP * STEP : b; };
@@ -537,21 +536,21 @@ struct Kv4Sums {
     while (b < b1) {
       const int bm = past(bn + STEP), idm = kv4_page_id(a, seq, bm, b1);
       if (idn >= 0) nxt.load(heads + idn * page_words + (size_t)(bn & 3) * kv4_block_words<HD>(), lane);
-      if (id >= 0) block<MASK>(raw, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane, mask, off);
+      if (id >= 0) block<MASK>(raw, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
       raw = nxt; b = bn; id = idn; bn = bm; idn = idm;
     }
   }
   // a wave's blocks (b_lo + first, in steps) of columns at positions p0 .. p1: those that every column sees whole, then the others
   template <int STEP>
-  __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, unsigned int* sp, int lane, unsigned int mask, unsigned int off) {
+  __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, unsigned int* sp, int lane) {
     // whole for every column: t0 + 31 <= p0 and t0 > p1 - window
     int w1 = (p0 + 1) >> 5, w0 = a.window > 0 && p1 - a.window + 1 > 0 ? (p1 - a.window + KV4_BLK) >> 5 : 0;
     w1 = min(max(w1, 0), b_hi);
     w0 = min(w0, w1);
     int f = first_block;
     if (f < w0) f += (w0 - f + STEP - 1) / STEP * STEP;
-    walk<false, STEP>(a, seq, kvh, f, w1, 0, 0, sp, lane, mask, off);
-    walk<true, STEP>(a, seq, kvh, first_block, b_hi, w0, w1, sp, lane, mask, off);
+    walk<false, STEP>(a, seq, kvh, f, w1, 0, 0, sp, lane);
+    walk<true, STEP>(a, seq, kvh, first_block, b_hi, w0, w1, sp, lane);
   }
 
   // o becomes the columns' sums, l their denominators (over the four quarters)
@@ -564,7 +563,7 @@ struct Kv4Sums {
         const float lg = kv4_sum_quarters(lov[t][g]);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const float add = fmaf(CENTRE ? -136.f : -128.f, ones[t][g][r], __shfl(lg, 4 * q4 + r, 64));
+          const float add = __shfl(lg, 4 * q4 + r, 64);
 #pragma unroll
           for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
         }
@@ -635,12 +634,10 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
   if (NT == 1) kv4_append_first<HD>(a, en, rg, kvh);
   const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  unsigned int mask = 0x000f000fu, off = 0x43004300u;      // (in registers: one instruction a pair with both)
-  asm("" : "+s"(mask), "+v"(off));
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
   Sums s;
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  s.template all<KW>(a, en.seq, kvh, b_lo + wv, b_hi, first, last, s_par[wv], lane, mask, off);
+  s.template all<KW>(a, en.seq, kvh, b_lo + wv, b_hi, first, last, s_par[wv], lane);
   s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -674,12 +671,10 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
   const int first = en.start + col0 / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
   const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  unsigned int mask = 0x000f000fu, off = 0x43004300u;
-  asm("" : "+s"(mask), "+v"(off));
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
   Sums s;
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  s.template all<1>(a, en.seq, kvh, b_lo, b_hi, first, last, s_par[wv], lane, mask, off);
+  s.template all<1>(a, en.seq, kvh, b_lo, b_hi, first, last, s_par[wv], lane);
   s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -729,8 +724,6 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   const Kv4Range rg = kv4_range(last, last, a.window, a.table_len, split, a.splits);
   kv4_append_first<HD>(a, en, rg, kvh);
   const int key_lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
-  unsigned int mask = 0x000f000fu, off = 0x43004300u;
-  asm("" : "+s"(mask), "+v"(off));
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5) & ~(NB - 1);      // (a step's blocks are of one page)
   const int tile = RPT == 4 ? q4 : q4 >> 1;                       // this lane's token of a step: 16 tile + n16, heads h0 .. h0 + 3
   const int h0 = RPT == 4 ? 0 : 4 * (q4 & 1);
@@ -777,9 +770,9 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
         u32x4 f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          f[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+          f[e] = pack_bf16(x[kv4_slot[2 * e]], x[kv4_slot[2 * e + 1]]);
           sum[ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
-          x[2 * e] -= bf16_lo(f[e]); x[2 * e + 1] -= bf16_hi(f[e]);
+          x[kv4_slot[2 * e]] -= bf16_lo(f[e]); x[kv4_slot[2 * e + 1]] -= bf16_hi(f[e]);
         }
         qf[ch][term] = __builtin_bit_cast(bf16x8_t, f);
       }
@@ -791,7 +784,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
       for (int r = 0; r < 4; r++) qs[g][r] = __shfl(t, h0 + r, 64);
     }
   }
-  f32x4 o[CT], ones[G];
+  f32x4 o[CT];
   float m[4], ref[4], l[4], lov[G][4];                            // references of the weights, in scores before the scale and (ref) negative behind it
 #pragma unroll
   for (int r = 0; r < 4; r++) {
@@ -801,10 +794,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   }
 #pragma unroll
   for (int c = 0; c < CT; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int g = 0; g < G; g++) ones[g] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bf16x8_t one8 = __builtin_bit_cast(bf16x8_t, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  const int w_at = (tile >> 1) * 32 + (n16 >> 2) * 8 + (n16 & 3) + 4 * (tile & 1);      // this lane's token among a head's weights
+  const int w_at = (tile >> 1) * 32 + (n16 >> 2) * 8 + 2 * (n16 & 3) + (tile & 1);      // this lane's token among a head's weights
   const float scale = a.scale_log2, gap = a.gap;
 
   // Steps: NB blocks each; what is not seen (or there) has levels of zero and a score of -inf.  The next step's keys are asked for when this one's are products, its values behind
@@ -830,18 +820,17 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           const int x = (t & 1) * CH + 2 * g + c;
-          const bf16x8_t kf = kv4_frag(rk[t >> 1][x >> 2][x & 3], mask, off);
+          const bf16x8_t kf = kv4_frag(rk[t >> 1][x >> 2][x & 3]);
 #pragma unroll
           for (int term = 0; term < TQ; term++) d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[2 * g + c][term], kf, d[t], 0, 0, 0);
         }
       }
-      const float z = fmaf(-128.f, st[0][g], lo[0][g]);
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         float v;
         if constexpr (RPT == 4) v = q4 < 2 ? (q4 == 0 ? d[0][r] : d[1][r]) : (q4 == 2 ? d[NJ - 2][r] : d[NJ - 1][r]);
         else v = q4 < 2 ? d[0][r] : d[1][r];
-        sc[r] = fmaf(st[0][g], v, fmaf(z, qs[g][r], g == 0 ? begin : sc[r]));
+        sc[r] = fmaf(st[0][g], v, fmaf(lo[0][g], qs[g][r], g == 0 ? begin : sc[r]));
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -864,7 +853,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
         m[r] = mx; ref[r] = -mx * scale;
         l[r] *= f;
 #pragma unroll
-        for (int g = 0; g < G; g++) { lov[g][r] *= f; ones[g][r] *= f; }
+        for (int g = 0; g < G; g++) lov[g][r] *= f;
 #pragma unroll
         for (int c = 0; c < CT; c++) o[c][r] *= f;
       }
@@ -900,13 +889,11 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
       wave_fence();
 #pragma unroll
       for (int x = 0; x < NB; x++) {
-#pragma unroll
-        for (int term = 0; term < TP; term++) ones[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], one8, ones[g], 0, 0, 0);
         bf16x8_t vf[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           const int i = 4 * g + c;
-          vf[c] = kv4_frag(rv[x][i >> 2][i & 3], mask, off);
+          vf[c] = kv4_frag(rv[x][i >> 2][i & 3]);
           o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][0], vf[c], o[i], 0, 0, 0);
         }
 #pragma unroll
@@ -933,9 +920,8 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
       w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false));
       t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
       if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false)); t = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
-      const float add = fmaf(-128.f, ones[g][r], t);
 #pragma unroll
-      for (int c = 0; c < 4; c++) o[4 * g + c][r] += add;
+      for (int c = 0; c < 4; c++) o[4 * g + c][r] += t;
     }
   }
   const int nv = a.group;

@@ -105,7 +105,7 @@ void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s) {
     else hipLaunchKernelGGL((tgx::kv4_read_kernel<128, DT>), grid, dim3(64), 0, s, a);)
 }
 
-template <int HD, int TQ, int TP, int TPC>
+template <int HD, int TQ, int TP>
 static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
   const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries);
   const size_t lds = (size_t)p.kw * std::min<long long>(16, (long long)a.max_count * a.group) * HD * 4;
@@ -118,7 +118,7 @@ static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStrea
   }
   else if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
   else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, TQ, TP>), grid, dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TPC>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TP>), grid, dim3(256), 0, s, a);
 }
 
 // a.splits, a.part, a.ml follow from the plan and the workspace here; with keys and values to append that the attention launch does not append itself, an append launch first
@@ -130,13 +130,13 @@ void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws,
   a.part = ws; a.ml = ws + rows * p.splits * hd;
   // terms of queries and weights by the outputs' type (kernels/kv4.h)
   if (hd == 64) {
-    if (a.q_dt == tgx::DT_BF16) launch_attend<64, 1, 2, 1>(a, p, s);
-    else if (a.q_dt == tgx::DT_F16) launch_attend<64, 2, 2, 2>(a, p, s);
-    else launch_attend<64, 3, 3, 3>(a, p, s);
+    if (a.q_dt == tgx::DT_BF16) launch_attend<64, 1, 2>(a, p, s);
+    else if (a.q_dt == tgx::DT_F16) launch_attend<64, 2, 2>(a, p, s);
+    else launch_attend<64, 3, 3>(a, p, s);
   } else {
-    if (a.q_dt == tgx::DT_BF16) launch_attend<128, 1, 2, 1>(a, p, s);
-    else if (a.q_dt == tgx::DT_F16) launch_attend<128, 2, 2, 2>(a, p, s);
-    else launch_attend<128, 3, 3, 3>(a, p, s);
+    if (a.q_dt == tgx::DT_BF16) launch_attend<128, 1, 2>(a, p, s);
+    else if (a.q_dt == tgx::DT_F16) launch_attend<128, 2, 2>(a, p, s);
+    else launch_attend<128, 3, 3>(a, p, s);
   }
   if (p.splits > 1) {
     const dim3 grid(a.heads, a.max_count, a.entries);
