@@ -112,23 +112,25 @@ __device__ __forceinline__ void kv4_append_one(const Kv4Args& a, unsigned int* p
   }
 }
 
-// Single tokens: a wave a (entry, kv head).
+// Few tokens: a wave a (entry, token, kv head).
 template <int HD>
 __global__ __launch_bounds__(64) void kv4_append_token_kernel(const Kv4Args a) {
-  const Kv4Entry en = kv4_entry(a, blockIdx.y);
-  if (en.count < 1 || en.start < 0) return;
-  unsigned int* page = kv4_page(a, en.seq, en.start >> KV_BLOCK_SHIFT, blockIdx.x, HD);
-  if (page) kv4_append_one<HD, false>(a, page, en.tok0, en.start, blockIdx.x);
+  const Kv4Entry en = kv4_entry(a, blockIdx.z);
+  const int i = blockIdx.y, pos = en.start + i;
+  if (i >= en.count || pos < 0) return;
+  unsigned int* page = kv4_page(a, en.seq, pos >> KV4_PAGE_SHIFT, blockIdx.x, HD);
+  if (page) kv4_append_one<HD, false>(a, page, en.tok0 + i, pos, blockIdx.x);
 }
 
-// Portions: a wave a (entry, block of 32 positions, kv head).  A lane takes a whole group of one token (32 tokens x HD / 64 groups x {key, value}): the levels need no
-// exchange.  The codes pass through LDS as bytes [token][channel], where a value word finds its eight tokens.
+// Portions: a workgroup of 2 HD threads a (entry, block of 32 positions, kv head).  Two neighbouring lanes take a group of one token, 32 channels each (32 tokens x HD / 64 groups x {key, value}):
+// one exchange between them gives the levels.  The values' codes pass through LDS as bytes [token][channel], where a value word finds its eight tokens.  Bound by memory where there is
+// enough of it (16 rows of 2048 tokens, eight heads of 128: 34 us, 4.9 TB/s) and by the way through one block where there is not (4.8 us; a lane a whole group 10.5).
 template <int HD, int DT>
-__global__ __launch_bounds__(64) void kv4_append_block_kernel(const Kv4Args a) {
-  constexpr int G = HD / 64, LS = HD / 4 + 1;                  // LDS row of a token in words
-  __shared__ unsigned int s[KV4_BLK * LS];
+__global__ __launch_bounds__(2 * HD) void kv4_append_block_kernel(const Kv4Args a) {
+  constexpr int G = HD / 64, LS = HD + 4;                      // bytes of a token in LDS
+  __shared__ __attribute__((aligned(16))) unsigned char s[KV4_BLK * LS];
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
-  const int kvh = blockIdx.x, lane = threadIdx.x;
+  const int kvh = blockIdx.x, tid = threadIdx.x;
   if (en.count < 1) return;
   const int s0 = max(en.start, 0), b = (s0 >> 5) + blockIdx.y;      // block of positions
   const int p0 = max(s0, b * KV4_BLK), p1 = min(en.start + en.count, (b + 1) * KV4_BLK);
@@ -136,72 +138,68 @@ __global__ __launch_bounds__(64) void kv4_append_block_kernel(const Kv4Args a) {
   unsigned int* page = kv4_page(a, en.seq, b >> 2, kvh, HD);
   if (!page) return;
   unsigned int* blk = page + (size_t)(b & 3) * kv4_block_words<HD>();
-#pragma unroll
-  for (int r = 0; r < G; r++) {
-    const int item = r * 64 + lane, val = item / (32 * G), rest = item % (32 * G), t = rest / G, g = rest % G, pos = b * KV4_BLK + t;
+  {
+    const int half = tid & 1, item = tid >> 1, val = item / (32 * G), rest = item % (32 * G), t = rest / G, g = rest % G, pos = b * KV4_BLK + t;
     const bool in = pos >= p0 && pos < p1;
-    const long long tok = en.tok0 + (in ? pos - en.start : p0 - en.start);      // (a lane without a token reads one that is there)
-    const int sp = in ? pos : p0;
-    const elem_t<DT>* src = static_cast<const elem_t<DT>*>(val ? a.v : a.k) + (val ? tok * a.v_ts + kvh * a.v_hs : tok * a.k_ts + kvh * a.k_hs) + (long long)(sp & (KV_BLOCK - 1)) * a.slot_s + g * 64;
-    float x[64];
-    const bool wide = ((reinterpret_cast<uintptr_t>(src) & 15) == 0);
-    if (wide) {
+    const int sp = in ? pos : p0;                               // (a lane without a token reads one that is there)
+    const long long tok = en.tok0 + sp - en.start;
+    const elem_t<DT>* src = static_cast<const elem_t<DT>*>(val ? a.v : a.k) + (val ? tok * a.v_ts + kvh * a.v_hs : tok * a.k_ts + kvh * a.k_hs) + (long long)(sp & (KV4_PAGE - 1)) * a.slot_s + g * 64 + 32 * half;
+    float x[32];
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) slice_unpack<DT>(load_slice<DT>(src, i), x + 8 * i);
+      for (int i = 0; i < 4; i++) slice_unpack<DT>(load_slice<DT>(src, i), x + 8 * i);
     } else {
 #pragma unroll
-      for (int i = 0; i < 64; i++) x[i] = elem_to_f32<DT>(src[i]);
+      for (int i = 0; i < 32; i++) x[i] = elem_to_f32<DT>(src[i]);
     }
     float mn = x[0], mx = x[0];
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 64; i++) { mn = fminf(mn, x[i]); mx = fmaxf(mx, x[i]); bad |= kv4_not_finite(x[i]); }
-    const Kv4Levels lv = kv4_levels(mn, mx, bad);
-    if (in) blk[kv4_param_word(HD, t, val, g)] = lv.word;
+    for (int i = 0; i < 32; i++) { mn = fminf(mn, x[i]); mx = fmaxf(mx, x[i]); bad |= kv4_not_finite(x[i]); }
+    mn = fminf(mn, dpp_mov<0xB1, 0xf>(mn));
+    mx = fmaxf(mx, dpp_mov<0xB1, 0xf>(mx));
+    const float wrong = bad ? 1.f : 0.f;
+    const Kv4Levels lv = kv4_levels(mn, mx, fmaxf(wrong, dpp_mov<0xB1, 0xf>(wrong)) != 0.f);
+    if (in && half == 0) blk[kv4_param_word(HD, t, val, g)] = lv.word;
     if (!val) {
 #pragma unroll
-      for (int c = 0; c < 2; c++)
+      for (int q = 0; q < 4; q++) {
+        unsigned int w = 0;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          unsigned int w = 0;
-#pragma unroll
-          for (int e = 0; e < 8; e++) w |= kv4_code(x[32 * c + 8 * q + e], lv) << kv4_code_bit(e);
-          if (in) blk[kv4_key_word(HD, t, 64 * g + 32 * c + 8 * q)] = w;
-        }
+        for (int e = 0; e < 8; e++) w |= kv4_code(x[8 * q + e], lv) << kv4_code_bit(e);
+        if (in) blk[kv4_key_word(HD, t, 64 * g + 32 * half + 8 * q)] = w;
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
+      for (int i = 0; i < 8; i++) {
         unsigned int w = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) w |= kv4_code(x[4 * i + e], lv) << (8 * e);
-        s[t * LS + g * 16 + i] = w;
+        *reinterpret_cast<unsigned int*>(s + t * LS + g * 64 + 32 * half + 4 * i) = w;
       }
     }
   }
   __syncthreads();
-  // value words: a lane takes four neighbouring channels of a quarter's eight tokens
+  // value words: a thread takes two neighbouring channels of a quarter's eight tokens
+  const int q = tid / (HD / 2), c2 = 2 * (tid % (HD / 2));
+  unsigned int w[2] = {0, 0}, m = 0;
 #pragma unroll
-  for (int u = 0; u < HD / 64; u++) {
-    const int item = u * 64 + lane, q = item / (HD / 4), c4 = item % (HD / 4);
-    unsigned int w[4] = {0, 0, 0, 0}, m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int t = kv4_value_token(q, e), pos = b * KV4_BLK + t, bit = kv4_code_bit(e);
-      const unsigned int cs = s[t * LS + c4];
-      if (pos >= p0 && pos < p1) {
-        m |= 15u << bit;
-#pragma unroll
-        for (int c = 0; c < 4; c++) w[c] |= ((cs >> (8 * c)) & 15u) << bit;
-      }
+  for (int e = 0; e < 8; e++) {
+    const int t = kv4_value_token(q, e), pos = b * KV4_BLK + t, bit = kv4_code_bit(e);
+    const unsigned int cs = *reinterpret_cast<const unsigned short*>(s + t * LS + c2);
+    if (pos >= p0 && pos < p1) {
+      m |= 15u << bit;
+      w[0] |= (cs & 15u) << bit;
+      w[1] |= ((cs >> 8) & 15u) << bit;
     }
+  }
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      unsigned int* dst = blk + kv4_value_word(HD, 4 * q, 4 * c4 + c);
-      if (m == 0xffffffffu) *dst = w[c];
-      else if (m) {
-        const unsigned int old = __hip_atomic_load(dst, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_fetch_xor(dst, (old ^ w[c]) & m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+  for (int c = 0; c < 2; c++) {
+    unsigned int* dst = blk + kv4_value_word(HD, 4 * q, c2 + c);
+    if (m == 0xffffffffu) *dst = w[c];
+    else if (m) {
+      const unsigned int old = __hip_atomic_load(dst, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_fetch_xor(dst, (old ^ w[c]) & m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
 }

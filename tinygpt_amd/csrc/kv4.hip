@@ -83,18 +83,20 @@ int blocks_of(int n) { return (n + 30) / 32 + 1; }
 
 }  // namespace
 
+// Few tokens a wave a (token, head), beyond 512 such waves a workgroup a block of 32 positions.  us tokens / blocks: one row, eight heads of 128, 16 tokens 4.0 / 4.8, 64 5.4 / 5.2, 512
+// 15.1 / 4.9; 16 rows, 2 4.4 / 5.1, 5 5.0 / 5.2, 16 7.5 / 5.3, 2048 461 / 34
 void kv4_launch_append(const tgx::Kv4Args& a, int hd, hipStream_t s) {
   if (!a.entries || !a.max_count) return;
-  if (a.max_count == 1) {
-    const dim3 grid(a.kv_heads, a.entries);
+  if (a.max_count == 1 || (long long)a.max_count * a.entries * a.kv_heads <= 512) {
+    const dim3 grid(a.kv_heads, a.max_count, a.entries);
     if (hd == 64) hipLaunchKernelGGL(tgx::kv4_append_token_kernel<64>, grid, dim3(64), 0, s, a);
     else hipLaunchKernelGGL(tgx::kv4_append_token_kernel<128>, grid, dim3(64), 0, s, a);
     return;
   }
   const dim3 grid(a.kv_heads, blocks_of(a.max_count), a.entries);
   TGX_DT_SWITCH(a.kv_dt,
-    if (hd == 64) hipLaunchKernelGGL((tgx::kv4_append_block_kernel<64, DT>), grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((tgx::kv4_append_block_kernel<128, DT>), grid, dim3(64), 0, s, a);)
+    if (hd == 64) hipLaunchKernelGGL((tgx::kv4_append_block_kernel<64, DT>), grid, dim3(128), 0, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_append_block_kernel<128, DT>), grid, dim3(256), 0, s, a);)
 }
 
 void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s) {
