@@ -404,7 +404,14 @@ TGX_API int64_t tgx_past_length(const tgx_ctx* ctx);
  *                       ran — tgx_decode refuses until then.
  * tgx_sample_row     == Sampler::sample on ONE row's logits; the id becomes that row's device-resident next token.
  * tgx_past_length_row   the row's own pastLength. */
+/* tgx_fork_row       row `dst` (a retired row, or the next free one) becomes a copy of live row `src`: length, current token, logits.  Paged caches
+ *                       (option kv.budget_tokens): whole blocks are shared until a row is reset, the block that goes on is copied, so that a fork costs at most one block
+ *                       of the pool; TGX_ERR_CONTEXT when none is free.  Several continuations of one prompt, or a prefix that several prompts share, at one prefill.
+ * tgx_resize_kv      the pools of a paged cache made larger or smaller while its rows live: blocks in use move together to the front of new pools (the old ones are given
+ *                       back afterwards, both exist for the copy).  TGX_ERR_CONTEXT when more blocks are in use, TGX_ERR_NOMEM when the memory is not there: nothing has changed then. */
 TGX_API int tgx_reset_row(tgx_ctx* ctx, int row);
+TGX_API int tgx_fork_row(tgx_ctx* ctx, int src, int dst);
+TGX_API int tgx_resize_kv(tgx_ctx* ctx, int budget_tokens);
 TGX_API int tgx_forward_row(tgx_ctx* ctx, int row, const int64_t* ids, int seq);
 TGX_API int tgx_sample_row(tgx_ctx* ctx, int row, const tgx_sampler_cfg* cfg, uint64_t seed, int64_t* out_id);
 TGX_API int64_t tgx_past_length_row(const tgx_ctx* ctx, int row);
@@ -558,6 +565,10 @@ TGX_API int tgx_set_logits(tgx_ctx* ctx, const float* logits, int batch);
  *                  tgx_reset_row / tgx_reset_cache; max_ctx stays the per-row limit.  A call that would need a block when none is free returns TGX_ERR_CONTEXT and
  *                  changes nothing (retire a row, retry).  Results are those of the unpaged cache, bit for bit on the same kernels (tests/test_hip_paged.py);
  *                  tgx_get_option "kv.free_tokens" = the unassigned blocks' worth of tokens (-1 when unpaged)
+ *   "kv.bits"      (default 16; set BEFORE tgx_finalize, with kv.budget_tokens; 16-bit storage dtypes) 4: the paged cache holds keys and values in 4 bits with two bfloat16 levels per
+ *                  64 channels (tgx_kv4_cache below has the format; 9/32 of the 16-bit cache's memory and traffic).  A prompt attends to its keys and values as computed and leaves them
+ *                  quantised; a step attends to the quantised ones, its own token's included.  kv.budget_tokens and kv.free_tokens keep their meaning.  tgx_read_kv gives the values that the cache
+ *                  holds, tgx_write_kv quantises (keys and values together)
  *   "attn.split_min", "attn.gqa_split_min", "attn.mfma", "stack.gemv", "stack.rec_step", "stack.line", "stack.gemm_wt", "mlstm.narrow", "attn.mix_groups", "ssd.min", "rec.min", "stack.conv_tiles"  (layered models) keys a workgroup walks from which a step of few
  *                  tokens divides them between workgroups (four thresholds: 128 on the matrix cores, 2048 on the lane kernels for latent rows, 1024 for grouped queries, counted in a
  *                  mask's span.  The first key sets all four, the second the grouped-query ones; a negative value brings the defaults back; tgx_get_option gives the

@@ -1,6 +1,7 @@
 """Operators on a 4-bit cache (tinygpt_amd.ops, kernels/kv4.h) against their definitions in 64 bits (kv4_util.py), bit for bit where the definition says which bits."""
 import numpy as np
 import pytest
+import torch as _torch   # here, not in a test: before any module's test loads the library, which then shares torch's HIP runtime
 
 from kv4_util import PAGE, attend, bound, quantise, values
 
@@ -11,8 +12,7 @@ EPS = {"bf16": 2.0 ** -7, "fp16": 2.0 ** -10, "fp32": 2.0 ** -23}
 
 @pytest.fixture(scope="module")
 def torch():
-    import torch
-    return torch
+    return _torch
 
 
 def dtype_of(torch, name):

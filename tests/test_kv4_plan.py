@@ -39,7 +39,7 @@ extern "C" int places(int hd) {
 extern "C" int entry(int seqs, int seq, int start, int o0, int o1, long long tokens, int max_count) {
   int off[2] = {o0, o1};
   Kv4Args a{};
-  a.seqs = seqs; a.seq = &seq; a.start = &start; a.offsets = off; a.tokens = tokens; a.max_count = max_count; a.entries = 1;
+  a.seqs = seqs; a.seq = &seq; a.start = &start; a.offsets = off; a.tokens = tokens; a.max_count = max_count; a.entries = 1; a.each = 1;
   const Kv4Entry n = kv4_entry(a, 0);
   if (n.count && (n.seq < 0 || n.seq >= seqs || n.tok0 < 0 || n.tok0 + n.count > tokens || n.count > max_count || (long long)n.start + n.count > 0x7fffffffLL)) return -1;
   return n.count;
@@ -203,3 +203,12 @@ def test_tensors_are_checked_before_the_library():
     for args in [(pool, table[0], table[0]), (pool[0], table[0], table[0])]:
         with pytest.raises(ValueError):
             ops.copy_pages(*args)
+
+
+def test_two_runtimes_are_refused():
+    from tinygpt_amd import ops
+    line = "7f0000000000-7f0000001000 r-xp 00000000 08:01 42    {}\n".format
+    one = [line("/opt/rocm/lib/libamdhip64.so.7"), line("/opt/rocm/lib/libamdhip64.so.7"), line("/lib/libc.so.6"), "7f00-7f10 rw-p 0 00:00 0\n"]
+    ops._one_runtime(one)
+    with pytest.raises(RuntimeError, match="before the first Model"):
+        ops._one_runtime(one + [line("/site/torch/lib/libamdhip64.so")])

@@ -7,6 +7,7 @@
 #include <climits>
 #include <cstring>
 #include "ctx.h"
+#include "kernels/kv4.h"
 #include "stack.h"
 
 static std::string g_create_err;
@@ -244,6 +245,7 @@ static void update_attn_modes(tgx_ctx* c, int n_positions, int rows_per_launch =
   const long long direct_lim = direct_limit(c, rpl, step), nw4_lim = nw4_limit(c, rpl, step);
   c->attn_direct = c->past + n_positions <= direct_lim;
   c->attn_nw4 = c->attn_direct && nw4_lim > 0 && c->past + n_positions <= nw4_lim;
+  c->kv4_keys = kv4_bucket(c->past + n_positions);
   c->attn_mfma = !c->attn_direct && c->past >= attn_mfma_threshold(c) && c->dt != tgx::DT_F32 && !(c->d.qk_norm && c->d.head_dim == 128 && c->qk_fuse);
 }
 
@@ -252,7 +254,7 @@ static void launch_decode_step(tgx_ctx* c, const tgx_sampler_cfg& cfg) {
     // rows per weight pass (option decode.step_rows: 32 or 64): batches beyond 32 rows take four activation blocks per skinny product (one pass over
     // the weights for up to 64 rows) instead of two passes of two blocks
     // (128 rows = eight blocks exist on the LDS-DMA ring kernel only: every product must then take stored terms, i.e. the attention a direct form that writes them)
-    const bool wide_ok = c->skinny_dma && c->skinny_dma_oproj >= 2 && c->attn_direct && c->dt != tgx::DT_F32;
+    const bool wide_ok = !c->kv4 && c->skinny_dma && c->skinny_dma_oproj >= 2 && c->attn_direct && c->dt != tgx::DT_F32;
     const int per = c->decode_step_rows > 64 && !wide_ok ? 64 : c->decode_step_rows;
     for (int row0 = 0; row0 < c->batch; row0 += per) launch_decode_step_mfma(c, row0, std::min(per, c->batch - row0), cfg);
     return;
@@ -307,7 +309,7 @@ static int ensure_step_graph(tgx_ctx* c, const tgx_sampler_cfg& cfg, bool want_m
   int hit = -1, victim = 0;
   for (int i = 0; i < 6; i++) {
     const tgx_ctx::GraphSet& g = c->graph_cache[i];
-    if (g.step && g.batch == c->batch && same_cfg(g.cfg, cfg) && g.direct == c->attn_direct && g.mfma == c->attn_mfma && g.nw4 == c->attn_nw4) { hit = i; break; }
+    if (g.step && g.batch == c->batch && same_cfg(g.cfg, cfg) && g.direct == c->attn_direct && g.mfma == c->attn_mfma && g.nw4 == c->attn_nw4 && (!c->kv4 || g.kv4_keys == c->kv4_keys)) { hit = i; break; }
     if (!g.step) victim = i;
     else if (c->graph_cache[victim].step && g.used < c->graph_cache[victim].used) victim = i;
   }
@@ -322,7 +324,7 @@ static int ensure_step_graph(tgx_ctx* c, const tgx_sampler_cfg& cfg, bool want_m
     }
     int rc = capture_steps(c, cfg, 1, &g.step);
     if (rc) { g = tgx_ctx::GraphSet{}; return rc; }
-    g.batch = c->batch; g.cfg = cfg; g.direct = c->attn_direct; g.mfma = c->attn_mfma; g.nw4 = c->attn_nw4;
+    g.batch = c->batch; g.cfg = cfg; g.direct = c->attn_direct; g.mfma = c->attn_mfma; g.nw4 = c->attn_nw4; g.kv4_keys = c->kv4_keys;
     g.used = ++c->graph_clock;
     hit = victim;
   }
@@ -357,7 +359,7 @@ int kv_ensure_blocks(tgx_ctx* c, int row, long long tokens) {
     return set_err(c, TGX_ERR_CONTEXT, "KV budget exhausted: row %d needs %d more blocks of %d tokens, %zu free of %d (option kv.budget_tokens = %d)", row, need - have,
                    tgx::KV_BLOCK, c->kv_free.size(), c->kv_nblocks - 1, c->kv_budget_tokens);
   std::vector<std::pair<int, int>> ch;
-  for (; have < need; have++) { ch.emplace_back(row * c->kv_tbl_stride + have, c->kv_free.back()); c->kv_free.pop_back(); }
+  for (; have < need; have++) { ch.emplace_back(row * c->kv_tbl_stride + have, c->kv_free.back()); c->kv_ref[(size_t)c->kv_free.back()] = 1; c->kv_free.pop_back(); }
   kv_tbl_push(c, ch);
   return TGX_OK;
 }
@@ -366,9 +368,56 @@ static void kv_release_row(tgx_ctx* c, int row) {       // the row's blocks back
   if (!c->kv_paged) return;
   int& have = c->kv_row_nblk[(size_t)row];
   std::vector<std::pair<int, int>> ch;
-  for (int b = 0; b < have; b++) { const int i = row * c->kv_tbl_stride + b; c->kv_free.push_back(c->kv_tbl_host[(size_t)i]); ch.emplace_back(i, 0); }
+  for (int b = 0; b < have; b++) { const int i = row * c->kv_tbl_stride + b, p = c->kv_tbl_host[(size_t)i]; if (--c->kv_ref[(size_t)p] == 0) c->kv_free.push_back(p); ch.emplace_back(i, 0); }
   have = 0;
   kv_tbl_push(c, ch);
+}
+
+// Copies of whole blocks, all layers, inside the pools: the pairs go to the device by value, sixteen at a time, in front of the launch that reads them
+struct KvPairs { int n; int from[16], to[16]; };
+static __global__ void kv_pairs_set_kernel(int* dst, KvPairs u) { if ((int)threadIdx.x < u.n) { dst[threadIdx.x] = u.from[threadIdx.x]; dst[16 + threadIdx.x] = u.to[threadIdx.x]; } }
+
+// the pools of a paged cache: one in 4 bits, or keys and values
+struct KvPools { int n; unsigned char* base[2]; long long page; };
+static KvPools kv_pools(const tgx_ctx* c) {
+  if (c->kv4) return KvPools{1, {(unsigned char*)c->kv4_pool, nullptr}, (long long)tgx::kv4_page_words(c->d.kv_heads, c->d.head_dim) * 4};
+  return KvPools{2, {c->slab_k, c->slab_v}, (long long)c->d.kv_heads * tgx::KV_BLOCK * c->d.head_dim * (long long)c->esz};
+}
+static void kv_copy_pages(tgx_ctx* c, const KvPools& from, long long from_pages, const KvPools& to, long long to_pages, const int* idx_from, const int* idx_to, int n) {
+  for (int i = 0; i < from.n; i++) {
+    tgx::CopyPagesArgs a{};
+    a.src = from.base[i]; a.dst = to.base[i]; a.page = from.page; a.src_pool = from.page * from_pages; a.dst_pool = to.page * to_pages; a.src_pages = from_pages; a.dst_pages = to_pages;
+    a.from = idx_from; a.to = idx_to; a.n = n;
+    launch_copy_pages(a, c->d.layers, c->stream);
+  }
+}
+static void kv_copy_blocks(tgx_ctx* c, const std::vector<std::pair<int, int>>& pairs) {
+  for (size_t i = 0; i < pairs.size(); i += 16) {
+    KvPairs u{};
+    u.n = (int)std::min<size_t>(16, pairs.size() - i);
+    for (int k = 0; k < u.n; k++) { u.from[k] = pairs[i + (size_t)k].first; u.to[k] = pairs[i + (size_t)k].second; }
+    hipLaunchKernelGGL(kv_pairs_set_kernel, dim3(1), dim3(64), 0, c->stream, c->kv_pairs, u);
+    kv_copy_pages(c, kv_pools(c), c->kv_nblocks, kv_pools(c), c->kv_nblocks, c->kv_pairs, c->kv_pairs + 16, u.n);
+  }
+}
+// the row's first n blocks are its own after this (tgx_write_kv: a fork may share them)
+static int kv_own_blocks(tgx_ctx* c, int row, int n) {
+  std::vector<std::pair<int, int>> pairs, ch;
+  n = std::min(n, c->kv_row_nblk[(size_t)row]);
+  size_t shared = 0;
+  for (int b = 0; b < n; b++) shared += c->kv_ref[(size_t)c->kv_tbl_host[(size_t)row * c->kv_tbl_stride + b]] > 1;
+  if (shared > c->kv_free.size()) return set_err(c, TGX_ERR_CONTEXT, "KV budget exhausted: %zu shared blocks of row %d to copy, %zu free", shared, row, c->kv_free.size());
+  for (int b = 0; b < n; b++) {
+    const int i = row * c->kv_tbl_stride + b, p = c->kv_tbl_host[(size_t)i];
+    if (c->kv_ref[(size_t)p] < 2) continue;
+    const int q = c->kv_free.back();
+    c->kv_free.pop_back();
+    c->kv_ref[(size_t)p]--; c->kv_ref[(size_t)q] = 1;
+    pairs.emplace_back(p, q); ch.emplace_back(i, q);
+  }
+  kv_copy_blocks(c, pairs);
+  kv_tbl_push(c, ch);
+  return TGX_OK;
 }
 
 // tgx_read_probs evaluates a row's final probabilities on demand: remember what its last sampled step was configured with
@@ -412,7 +461,7 @@ static int run_decode_steps(tgx_ctx* c, const tgx_sampler_cfg& cfg, uint64_t see
   int remaining = n;
   while (remaining > 0) {
     int m = remaining;
-    const long long lims[2] = {nw4_limit(c, c->batch, true), direct_limit(c, c->batch, true)};
+    const long long lims[3] = {nw4_limit(c, c->batch, true), direct_limit(c, c->batch, true), c->kv4 ? kv4_bucket(c->past + 1) : 0};
     for (long long lim : lims)
       if (lim > 0 && c->past + 1 <= lim && c->past + m > lim) m = (int)(lim - c->past);
     update_attn_modes(c, m);
@@ -667,6 +716,7 @@ int tgx_finalize(tgx_ctx* c) {
   size_t kv_elems = (size_t)d.layers * d.kv_heads * d.max_ctx * hd;
   c->kv_row_elems = kv_elems;
   size_t kv_total = B * kv_elems;                     // elements of the K cache (and of the V cache)
+  if (c->kv_bits == 4 && c->kv_budget_tokens <= 0) return set_err(c, TGX_ERR_UNSUPPORTED, "kv.bits 4: with kv.budget_tokens (a paged cache)");
   if (c->kv_budget_tokens > 0) {                      // paged KV: pools of KV_BLOCK-token blocks shared by the rows (kernels/common.h)
     if (c->dt == tgx::DT_F32) return set_err(c, TGX_ERR_UNSUPPORTED, "kv.budget_tokens: paged KV serves the 16-bit storage dtypes");
     c->kv_paged = true;
@@ -678,6 +728,13 @@ int tgx_finalize(tgx_ctx* c) {
     HIP_OK(c, hipMemset(c->kv_tbl, 0, B * (size_t)c->kv_tbl_stride * 4));
     c->kv_tbl_host.assign(B * (size_t)c->kv_tbl_stride, 0);
     c->kv_row_nblk.assign(B, 0);
+    c->kv_ref.assign((size_t)c->kv_nblocks, 0);
+    if ((rc = dev_alloc(c, &c->kv_pairs, 32))) return rc;
+    if (c->kv_bits == 4) {                            // pages in 4 bits; slab_k / slab_v: one 16-bit staging block a row, for all layers in turn
+      c->kv4 = true;
+      kv_total = B * (size_t)d.kv_heads * tgx::KV_BLOCK * hd;
+      if ((rc = kv4_alloc(c))) return rc;
+    }
     c->kv_free.clear();
     for (int b = c->kv_nblocks - 1; b >= 1; b--) c->kv_free.push_back(b);
   }
@@ -710,6 +767,7 @@ int tgx_finalize(tgx_ctx* c) {
     r.tok = c->slab_tok + b; r.pos = c->slab_pos + b; r.prompt = c->slab_prompt + b * d.max_ctx;
     r.kcache = c->slab_k + b * kv_elems * c->esz; r.vcache = c->slab_v + b * kv_elems * c->esz;
     if (c->kv_paged) { r.kcache = c->slab_k; r.vcache = c->slab_v; r.tbl = c->kv_tbl + b * (size_t)c->kv_tbl_stride; }
+    if (c->kv4) { r.tbl4 = r.tbl; r.tbl = c->kv4_stage_tbl + b * (size_t)c->kv_tbl_stride; }
   }
   if ((rc = dev_alloc(c, &c->ch_x, 4 * (size_t)H))) return rc;
   if ((rc = dev_alloc(c, &c->ch_q, 4 * (size_t)qd))) return rc;
@@ -756,7 +814,7 @@ void tgx_destroy(tgx_ctx* c) {
   stack_destroy(c);
   auto fr = [](void* p) { if (p) (void)hipFree(p); };
   fr(c->embed); fr(c->lm_head); fr(c->final_norm); fr(c->wpe); fr(c->final_norm_b); fr(c->rope_cos); fr(c->rope_sin); fr(c->step); fr(c->step_done); fr(c->tok_log); fr(c->scratch_x); fr(c->seed_dev); fr(c->samp_scratch); fr(c->samp_list_comp); fr(c->samp_list_v);
-  fr(c->slab_acc); fr(c->kv_tbl);
+  fr(c->slab_acc); fr(c->kv_tbl); fr(c->kv_pairs); fr(c->kv4_pool); fr(c->kv4_stage_tbl); fr(c->kv4_prompt_tbl); fr(c->kv4_zero); fr(c->kv4_pk); fr(c->kv4_pv); fr(c->kv4_ws);
   fr(c->ch_x); fr(c->ch_q); fr(c->ch_kraw); fr(c->ch_attn); fr(c->ch_h); fr(c->ch_part); fr(c->ch_pos);
   fr(c->ws_x); fr(c->ws_out); fr(c->ws_ah); fr(c->ws_al); fr(c->ws_al2); fr(c->ws_qh); fr(c->ws_ql); fr(c->ws_hh); fr(c->ws_hl); fr(c->ws_part); fr(c->ws_ssq); fr(c->ws_pos);
   for (auto& w : c->L) { fr(w.in_norm); fr(w.post_norm); fr(w.wqkv); fr(w.bqkv); fr(w.wo); fr(w.q_norm); fr(w.k_norm); fr(w.wgu); fr(w.wdown); fr(w.in_norm_b); fr(w.post_norm_b); fr(w.bo); fr(w.bfc); fr(w.bdown); }
@@ -806,8 +864,10 @@ int tgx_forward(tgx_ctx* c, const int64_t* ids, int batch, int seq) {
       int rc = skinny ? ensure_skinny_ws(c, nb * seq) : ensure_prefill_ws(c, nb * seq);
       if (rc) return rc;
       if (f32_path && (rc = ensure_f32_part(c, nb * seq))) return rc;
+      if (c->kv4 && (rc = kv4_prompt_begin(c, row0, nb, seq))) return rc;
       if (f32_path) launch_prefill_f32(c, row0, nb, seq);
       else if (skinny) launch_prefill_skinny(c, row0, nb, seq); else launch_prefill(c, row0, nb, seq, (int)c->past);   // tgx_forward: every row at the batch's pastLength
+      if (c->kv4) kv4_prompt_end(c, row0, nb);
       for (int b = row0; b < row0 + nb;) {
         const int rem = row0 + nb - b, R = rem >= 4 ? 4 : (rem >= 2 ? 2 : 1);
         launch_lm_head(c, b, R);
@@ -825,7 +885,7 @@ int tgx_forward(tgx_ctx* c, const int64_t* ids, int batch, int seq) {
     for (int s0 = 0; s0 < seq;) {
       const int rem = seq - s0, R = rem >= 4 ? 4 : (rem >= 2 ? 2 : 1);
       launch_embed_chunk(c, r.prompt + s0, R, (int)c->past + s0);
-      for (int k = 0; k < R; k++) { c->chunk[k].kcache = r.kcache; c->chunk[k].vcache = r.vcache; c->chunk[k].tbl = r.tbl; }
+      for (int k = 0; k < R; k++) { c->chunk[k].kcache = r.kcache; c->chunk[k].vcache = r.vcache; c->chunk[k].tbl = r.tbl; c->chunk[k].tbl4 = r.tbl4; }
       launch_layers(c, c->chunk, R, 0);
       s0 += R;
       if (s0 == seq) {                                   // the last position's hidden state feeds lm_head; publish token and length
@@ -1038,9 +1098,11 @@ int tgx_forward_row(tgx_ctx* c, int row, const int64_t* ids, int seq) {
                         (seq <= 32 ? c->prefill_skinny_rows >= seq : (seq <= c->prefill_skinny_rows && c->d.hidden <= c->prefill_skinny_hidden_max && (seq <= 64 || (c->skinny_dma && c->d.hidden <= c->prefill_skinny_hidden_max_wide))));
     rc = skinny ? ensure_skinny_ws(c, seq) : ensure_prefill_ws(c, seq);
     if (!rc && f32_path) rc = ensure_f32_part(c, seq);
+    if (!rc && c->kv4) rc = kv4_prompt_begin(c, row, 1, seq);
     if (!rc) {
       if (f32_path) launch_prefill_f32(c, row, 1, seq);
       else if (skinny) launch_prefill_skinny(c, row, 1, seq); else launch_prefill(c, row, 1, seq, /*past=*/0);
+      if (c->kv4) kv4_prompt_end(c, row, 1);
       launch_lm_head(c, row, 1);
       launch_add_pos(c, r.pos, seq);
     }
@@ -1049,7 +1111,7 @@ int tgx_forward_row(tgx_ctx* c, int row, const int64_t* ids, int seq) {
     for (int s0 = 0; s0 < seq;) {
       const int rem = seq - s0, R = rem >= 4 ? 4 : (rem >= 2 ? 2 : 1);
       launch_embed_chunk(c, r.prompt + s0, R, s0);
-      for (int k = 0; k < R; k++) { c->chunk[k].kcache = r.kcache; c->chunk[k].vcache = r.vcache; c->chunk[k].tbl = r.tbl; }
+      for (int k = 0; k < R; k++) { c->chunk[k].kcache = r.kcache; c->chunk[k].vcache = r.vcache; c->chunk[k].tbl = r.tbl; c->chunk[k].tbl4 = r.tbl4; }
       launch_layers(c, c->chunk, R, 0);
       s0 += R;
       if (s0 == seq) {
@@ -1101,6 +1163,108 @@ int tgx_sample_row(tgx_ctx* c, int row, const tgx_sampler_cfg* cfg, uint64_t see
   refresh_longest(c);
   return TGX_OK;
 }
+
+int tgx_fork_row(tgx_ctx* c, int src, int dst) {
+  if (!c) return TGX_ERR_INVALID;
+  if (!c->finalized) return set_err(c, TGX_ERR_STATE, "fork before finalize");
+  if (c->stack || !c->kv_paged) return set_err(c, TGX_ERR_UNSUPPORTED, "tgx_fork_row serves the flat families with a paged cache (option kv.budget_tokens)");
+  if (c->poisoned) return set_err(c, TGX_ERR_STATE, "an earlier pass failed half-way: call tgx_reset_cache first");
+  if (src < 0 || src >= c->batch || c->row_idle[(size_t)src] || c->row_past[(size_t)src] <= 0) return set_err(c, TGX_ERR_INVALID, "row %d holds no sequence to fork", src);
+  if (dst < 0 || dst >= c->d.max_batch || dst > c->batch || dst == src) return set_err(c, TGX_ERR_INVALID, "row %d: a retired row [0,%d) or the next free one (max_batch %d)", dst, c->batch, c->d.max_batch);
+  if (dst < c->batch && !c->row_idle[(size_t)dst]) return set_err(c, TGX_ERR_STATE, "row %d holds %lld positions: tgx_reset_row first", dst, (long long)c->row_past[(size_t)dst]);
+  HIP_OK(c, hipSetDevice(c->device));
+  // whole blocks are shared (a row writes behind its length only); the one that goes on is copied, in every layer
+  const int64_t past = c->row_past[(size_t)src];
+  const int whole = (int)(past / tgx::KV_BLOCK), part = past % tgx::KV_BLOCK ? 1 : 0;
+  kv_release_row(c, dst);
+  if (part && c->kv_free.empty()) return set_err(c, TGX_ERR_CONTEXT, "KV budget exhausted: a fork of row %d needs a block of %d tokens, none is free (option kv.budget_tokens = %d)", src, tgx::KV_BLOCK, c->kv_budget_tokens);
+  std::vector<std::pair<int, int>> ch;
+  for (int b = 0; b < whole + part; b++) {
+    int p = c->kv_tbl_host[(size_t)src * c->kv_tbl_stride + b];
+    if (b == whole) {
+      const int q = c->kv_free.back();
+      c->kv_free.pop_back();
+      kv_copy_blocks(c, {{p, q}});
+      p = q;
+    }
+    c->kv_ref[(size_t)p]++;
+    ch.emplace_back(dst * c->kv_tbl_stride + b, p);
+  }
+  c->kv_row_nblk[(size_t)dst] = whole + part;
+  kv_tbl_push(c, ch);
+  // the row's own: position, current token and its embedding row, logits with the partials that the greedy choice reads
+  const RowState &f = c->rows[(size_t)src], &t = c->rows[(size_t)dst];
+  struct { void* to; const void* from; size_t n; } own[] = {{t.pos, f.pos, 4}, {t.tok, f.tok, 4}, {t.x, f.x, (size_t)c->d.hidden * 4}, {t.logits, f.logits, (size_t)c->d.vocab * 4},
+                                                            {t.part_val, f.part_val, (size_t)c->lm_grid * 4}, {t.part_idx, f.part_idx, (size_t)c->lm_grid * 4}};
+  for (const auto& m : own) HIP_OK(c, hipMemcpyAsync(m.to, m.from, m.n, hipMemcpyDeviceToDevice, c->stream));
+  HIP_OK(c, hipGetLastError());
+  c->batch = std::max(c->batch, dst + 1);
+  c->row_past[(size_t)dst] = past;
+  c->row_tok[(size_t)dst] = c->row_tok[(size_t)src];
+  c->row_idle[(size_t)dst] = 0;
+  if ((size_t)dst < c->row_probs_ok.size()) c->row_probs_ok[(size_t)dst] = 0;
+  refresh_longest(c);
+  return TGX_OK;
+}
+
+int tgx_resize_kv(tgx_ctx* c, int budget_tokens) {
+  if (!c) return TGX_ERR_INVALID;
+  if (!c->finalized) return set_err(c, TGX_ERR_STATE, "resize before finalize (option kv.budget_tokens sizes the cache)");
+  if (c->stack || !c->kv_paged) return set_err(c, TGX_ERR_UNSUPPORTED, "tgx_resize_kv serves the flat families with a paged cache (option kv.budget_tokens)");
+  if (budget_tokens < 1) return set_err(c, TGX_ERR_INVALID, "budget_tokens %d", budget_tokens);
+  HIP_OK(c, hipSetDevice(c->device));
+  const tgx_model_desc& d = c->d;
+  const int blocks = (int)(((long long)budget_tokens + tgx::KV_BLOCK - 1) / tgx::KV_BLOCK) + 1;
+  // blocks in use move to the front of the new pools, in the order of their numbers
+  std::vector<int> where((size_t)c->kv_nblocks, 0), from, to;
+  for (int p = 1; p < c->kv_nblocks; p++)
+    if (c->kv_ref[(size_t)p] > 0) { from.push_back(p); to.push_back((int)from.size()); where[(size_t)p] = (int)from.size(); }
+  if ((int)from.size() > blocks - 1) return set_err(c, TGX_ERR_CONTEXT, "%zu blocks of %d tokens are in use, a budget of %d tokens has %d", from.size(), tgx::KV_BLOCK, budget_tokens, blocks - 1);
+  const KvPools old = kv_pools(c);
+  KvPools now = old;
+  int* idx = nullptr;
+  const size_t bytes = (size_t)d.layers * blocks * (size_t)old.page;
+  hipError_t e = hipSuccess;
+  for (int i = 0; i < now.n; i++) now.base[i] = nullptr;
+  for (int i = 0; i < now.n && e == hipSuccess; i++) e = hipMalloc((void**)&now.base[i], bytes);
+  if (e == hipSuccess && !from.empty()) e = hipMalloc((void**)&idx, 2 * from.size() * 4);
+  if (e != hipSuccess) {      // everything stays as it was
+    (void)hipGetLastError();
+    for (int i = 0; i < now.n; i++) if (now.base[i]) (void)hipFree(now.base[i]);
+    return set_err(c, TGX_ERR_NOMEM, "%zu bytes of device memory: %s", bytes * (size_t)now.n, hipGetErrorString(e));
+  }
+  drop_step_graphs(c);
+  for (int i = 0; i < now.n && e == hipSuccess; i++) e = hipMemsetAsync(now.base[i], 0, bytes, c->stream);
+  if (e == hipSuccess && idx) {
+    e = hipMemcpy(idx, from.data(), from.size() * 4, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipMemcpy(idx + from.size(), to.data(), to.size() * 4, hipMemcpyHostToDevice);
+    if (e == hipSuccess) {
+      for (size_t i = 0; i < from.size(); i += 32768) kv_copy_pages(c, old, c->kv_nblocks, now, blocks, idx + i, idx + from.size() + i, (int)std::min<size_t>(32768, from.size() - i));
+      e = hipGetLastError();
+    }
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+  if (idx) (void)hipFree(idx);
+  if (e != hipSuccess) {
+    for (int i = 0; i < now.n; i++) (void)hipFree(now.base[i]);
+    return set_err(c, TGX_ERR_DEVICE, "resize: %s", hipGetErrorString(e));
+  }
+  for (int i = 0; i < old.n; i++) (void)hipFree(old.base[i]);
+  if (c->kv4) c->kv4_pool = (unsigned int*)now.base[0];
+  else {
+    c->slab_k = now.base[0]; c->slab_v = now.base[1];
+    for (auto& r : c->rows) { r.kcache = c->slab_k; r.vcache = c->slab_v; }
+  }
+  std::vector<int> ref((size_t)blocks, 0);
+  for (size_t i = 0; i < from.size(); i++) ref[(size_t)to[i]] = c->kv_ref[(size_t)from[i]];
+  c->kv_ref = ref;
+  for (auto& t : c->kv_tbl_host) t = where[(size_t)t];
+  c->kv_free.clear();
+  for (int b = blocks - 1; b > (int)from.size(); b--) c->kv_free.push_back(b);
+  c->kv_nblocks = blocks; c->kv_budget_tokens = budget_tokens;
+  HIP_OK(c, hipMemcpy(c->kv_tbl, c->kv_tbl_host.data(), c->kv_tbl_host.size() * 4, hipMemcpyHostToDevice));
+  return TGX_OK;
+}
 int64_t tgx_context_size(const tgx_ctx* c) { return c ? c->d.max_ctx : -1; }
 int32_t tgx_num_layers(const tgx_ctx* c) { return c ? c->d.layers : -1; }
 
@@ -1126,6 +1290,7 @@ int tgx_read_kv(tgx_ctx* c, int row, int layer, float* k_out, float* v_out) {
   HIP_OK(c, hipStreamSynchronize(c->stream));
   const tgx_model_desc& d = c->d;
   const size_t hd = (size_t)d.head_dim, per_head = (size_t)d.max_ctx * hd, T = (size_t)tgx_past_length_row(c, row);
+  if (c->kv4) return kv4_read_rows(c, row, layer, k_out, v_out, T);
   std::vector<unsigned char> tmp(per_head * c->esz);
   for (int which = 0; which < 2; which++) {
     float* out = which ? v_out : k_out;
@@ -1161,6 +1326,11 @@ int tgx_write_kv(tgx_ctx* c, int row, int layer, const float* k_in, const float*
   HIP_OK(c, hipStreamSynchronize(c->stream));
   const tgx_model_desc& d = c->d;
   const size_t hd = (size_t)d.head_dim, per_head = (size_t)d.max_ctx * hd, T = (size_t)n_rows;
+  if (c->kv_paged) { int rc = kv_own_blocks(c, row, (int)((T + tgx::KV_BLOCK - 1) / tgx::KV_BLOCK)); if (rc) return rc; HIP_OK(c, hipStreamSynchronize(c->stream)); }
+  if (c->kv4) {
+    if (!k_in || !v_in) return set_err(c, TGX_ERR_UNSUPPORTED, "tgx_write_kv: a cache in 4 bits takes keys and values together");
+    return kv4_write_rows(c, row, layer, k_in, v_in, T);
+  }
   std::vector<unsigned char> tmp(T * hd * c->esz);
   for (int which = 0; which < 2; which++) {
     const float* in = which ? v_in : k_in;
@@ -1272,6 +1442,7 @@ int tgx_get_option(const tgx_ctx* c, const char* key, int* out_value) {
   if (!strcmp(key, "graph.steps")) { *out_value = c->graph_steps; return TGX_OK; }
   if (!strcmp(key, "act.round16")) { *out_value = c->act16; return TGX_OK; }
   if (!strcmp(key, "kv.budget_tokens")) { *out_value = c->kv_budget_tokens; return TGX_OK; }
+  if (!strcmp(key, "kv.bits")) { *out_value = c->dt == tgx::DT_F32 ? 32 : c->kv_bits; return TGX_OK; }
   if (!strcmp(key, "kv.free_tokens")) { *out_value = c->kv_paged ? (int)c->kv_free.size() * tgx::KV_BLOCK : -1; return TGX_OK; }      // paged KV: tokens' worth of unassigned blocks
   return TGX_ERR_INVALID;
 }
@@ -1364,6 +1535,12 @@ int tgx_set_option(tgx_ctx* c, const char* key, int value) {
     if (value < 0) return set_err(c, TGX_ERR_INVALID, "kv.budget_tokens >= 0 (0 = one max_ctx slab per row)");
     c->kv_budget_tokens = value; return TGX_OK;
   }
+  if (!strcmp(key, "kv.bits")) {
+    if (c->finalized) return set_err(c, TGX_ERR_STATE, "kv.bits is set before tgx_finalize (it sizes the caches)");
+    if (value != 4 && value != 16) return set_err(c, TGX_ERR_INVALID, "kv.bits is 16 (the storage dtype) or 4");
+    if (c->dt == tgx::DT_F32) return set_err(c, TGX_ERR_UNSUPPORTED, "kv.bits: the 16-bit storage dtypes");
+    c->kv_bits = value; return TGX_OK;
+  }
   if (!strcmp(key, "attn.nsplit")) {
     if (c->finalized) return set_err(c, TGX_ERR_STATE, "attn.nsplit must be set before tgx_finalize");
     if (value < 1 || value > 32) return set_err(c, TGX_ERR_INVALID, "attn.nsplit out of range");
@@ -1394,12 +1571,13 @@ int64_t tgx_bytes_per_token(const tgx_ctx* c, int64_t T) {
   const tgx_model_desc& d = c->d;
   const int64_t H = d.hidden, I = d.inter, V = d.vocab, L = d.layers, q = (int64_t)d.heads * d.head_dim, kv = (int64_t)d.kv_heads * d.head_dim;
   const int64_t b = (int64_t)c->esz;   // bytes per stored parameter / cache element
+  const int64_t cache = c->kv4 ? L * kv * T * 9 / 8 : b * 2 * L * kv * T;      // keys and values of T tokens (in 4 bits with their levels: 9 eighths of a byte a channel of both)
   if (c->gpt2) {   // c_attn, c_proj, c_fc, mlp.c_proj with their biases, two LayerNorms (weight + bias); ln_f, one wpe row, the wte head
     const int64_t per_layer = 3 * H * H + 3 * H + H * H + H + I * H + I + H * I + H + 4 * H;
-    return b * (L * per_layer + 2 * H + H + V * H) + b * 2 * L * kv * T;
+    return b * (L * per_layer + 2 * H + H + V * H) + cache;
   }
   const int64_t per_layer = (q + 2 * kv) * H + (d.qkv_bias ? (q + 2 * kv) : 0) + H * q + 2 * I * H + H * I + 2 * H;
-  return b * (L * per_layer + H + V * H) + b * 2 * L * kv * T;
+  return b * (L * per_layer + H + V * H) + cache;
 }
 
 }  // extern "C"

@@ -60,7 +60,8 @@ struct RowState {       // independent KV/sequence state of one batch row
   int *tok = nullptr, *pos = nullptr;
   long long* prompt = nullptr;
   ebyte *kcache = nullptr, *vcache = nullptr;   // [layers][kv_heads][max_ctx][hd] in the compute dtype; paged KV: the pools [layers][blocks][kv_heads][KV_BLOCK][hd], shared by the rows
-  const int* tbl = nullptr;                     // paged KV: this row's block table on the device
+  const int* tbl = nullptr;                     // paged KV: this row's block table on the device (a cache in 4 bits: of its staging blocks)
+  const int* tbl4 = nullptr;                    // a cache in 4 bits: this row's table of pages
 };
 
 struct Tune {
@@ -132,7 +133,7 @@ struct tgx_ctx {
   hipGraphExec_t multi_graph = nullptr;   // graph_steps consecutive decode steps (tgx_decode with many steps)
   // captured step graphs by (batch, sampler config, attention form): a generation that crosses an attention-form limit, or an engine that alternates between
   // sampler configurations / batch sizes, re-uses what it captured before instead of re-capturing (round 3; round 2 dropped the graphs at every change)
-  struct GraphSet { hipGraphExec_t step = nullptr, multi = nullptr; int batch = 0; tgx_sampler_cfg cfg{}; bool direct = false, mfma = false, nw4 = false; unsigned long long used = 0; };
+  struct GraphSet { hipGraphExec_t step = nullptr, multi = nullptr; int batch = 0; tgx_sampler_cfg cfg{}; bool direct = false, mfma = false, nw4 = false; int kv4_keys = 0; unsigned long long used = 0; };
   GraphSet graph_cache[6];
   unsigned long long graph_clock = 0;
   int graph_cur = -1;
@@ -255,6 +256,19 @@ struct tgx_ctx {
   std::vector<int> kv_tbl_host;    // its host mirror
   std::vector<int> kv_free;        // free physical blocks
   std::vector<int> kv_row_nblk;    // blocks assigned to each row
+  std::vector<int> kv_ref;         // rows that hold each physical block (tgx_fork_row: whole blocks are shared, the last one is copied)
+  int* kv_pairs = nullptr;         // device [2][16]: page copies of a fork
+  // ---- the cache in 4 bits (option kv.bits 4, with kv.budget_tokens; kernels/kv4.h).  kv_tbl names pages of kv4_pool; slab_k / slab_v hold one 16-bit staging block a row, which every launch that
+  // appends to the cache writes through kv4_stage_tbl (all of a row's entries name its block) without knowing of it, and from which the attention of a step takes the token's key and value
+  // into their page.  A prompt's pass has staging blocks for all its tokens, of one layer: its attention reads them, an append quantises them, the next layer writes them again.
+  int kv_bits = 16;
+  bool kv4 = false;
+  unsigned int* kv4_pool = nullptr;                     // [layers][kv_nblocks] pages
+  int *kv4_stage_tbl = nullptr, *kv4_prompt_tbl = nullptr, *kv4_zero = nullptr;
+  ebyte *kv4_pk = nullptr, *kv4_pv = nullptr;           // a prompt's staging blocks (grown to the longest pass)
+  size_t kv4_prompt_blocks = 0;
+  float* kv4_ws = nullptr; size_t kv4_ws_floats = 0;    // records of divided keys
+  int kv4_keys = 256;                                   // keys that a step's attention is divided for: a power of two, part of a captured step's identity
   long long* slab_acc = nullptr;   // [max_batch][hidden], resting at zero between layers
   float* scratch_x = nullptr;   // [hidden] residual sink for tgx_profile_decode
   Profiler prof;
@@ -304,6 +318,11 @@ namespace tgx { struct AttnArgs; struct FinalizeArgs; struct AttnPrefillArgs; st
 // ---- abi.hip
 void drop_step_graphs(tgx_ctx* c);
 int copy_to_host(tgx_ctx* c, void* dst, const void* src, size_t bytes);      // device memory to any host memory behind what the stream holds; there when it returns
+// elements between a layer's caches: a row's slab, or - paged - the layer's pool of blocks, or - a cache in 4 bits - none: the staging blocks serve every layer in turn
+inline size_t kv_layer_elems(const tgx_ctx* c) {
+  const size_t per = (size_t)c->d.kv_heads * c->d.head_dim;
+  return c->kv4 ? 0 : c->kv_paged ? per * c->kv_nblocks * tgx::KV_BLOCK : per * c->d.max_ctx;
+}
 int kv_ensure_blocks(tgx_ctx* c, int row, long long tokens);       // paged KV: row `row` may hold `tokens` tokens after this (assigns blocks, updates the device table, stream-ordered)
 bool is_greedy(const tgx_sampler_cfg* s);   // Sampler.cpp:15-21
 // ---- decode.hip (kernels/gemv.h, kernels/oproj_sliced.h)
@@ -353,3 +372,12 @@ void kv4_launch_append(const tgx::Kv4Args& a, int hd, hipStream_t s);
 void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s);
 void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws, hipStream_t s);
 void launch_copy_pages(const tgx::CopyPagesArgs& a, int layers, hipStream_t s);
+// a context's cache in 4 bits
+inline int kv4_bucket(long long keys) { int b = 256; while (b < keys && b < (1 << 30)) b *= 2; return b; }
+int kv4_alloc(tgx_ctx* c);                                              // pools, tables and workspace (tgx_finalize)
+int kv4_prompt_begin(tgx_ctx* c, int row0, int NB, int S);              // rows [row0, row0 + NB) write their prompts of S tokens to staging blocks ...
+void kv4_prompt_append(tgx_ctx* c, int l, int row0, int NB, int S);     // ... from which layer l's keys and values go to their pages ...
+void kv4_prompt_end(tgx_ctx* c, int row0, int NB);                      // ... until the rows are back to steps
+void kv4_step_attend(tgx_ctx* c, RowState* rv, int R, int l, bool one_sequence);
+int kv4_read_rows(tgx_ctx* c, int row, int layer, float* k_out, float* v_out, size_t T);
+int kv4_write_rows(tgx_ctx* c, int row, int layer, const float* k_in, const float* v_in, size_t T);

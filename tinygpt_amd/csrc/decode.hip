@@ -96,7 +96,7 @@ static void fill_strides(const tgx_ctx* c, tgx::GemvArgs& a) {
 
 // Qwen3: independent batch rows (each its own cache) take the q/k norm inside the attention launch; the positions of one sequence that a
 // prefill-by-steps pass handles together (kv_stride 0) need each other's finished keys, so they keep the separate norm launch
-static bool qk_fused(const tgx_ctx* c, long long kv_stride) { return c->d.qk_norm && c->d.head_dim == 128 && kv_stride != 0 && c->qk_fuse; }
+static bool qk_fused(const tgx_ctx* c, long long kv_stride) { return !c->kv4 && c->d.qk_norm && c->d.head_dim == 128 && kv_stride != 0 && c->qk_fuse; }
 
 // The K-sliced o_proj with the attention merge in its prologue (kernels/oproj_sliced.h; no attn_combine launch, fixed-point residual stream between o_proj
 // and down) serves batch-1 steps on the VALU split attention form: head_dim 64 (a slice of 2-4 heads reads 9-35 KB of records; at head_dim 128 the records
@@ -105,7 +105,7 @@ static bool qk_fused(const tgx_ctx* c, long long kv_stride) { return c->d.qk_nor
 // {attention, combine, o_proj} 12.9 -> {attention, sliced o_proj} 10.2 us per layer; Qwen2.5-0.5B 10.1 -> 8.4 (profiles/r04_oproj_sliced.txt).
 bool oproj_sliced_ok(const tgx_ctx* c, int R, long long kv_stride) {
   const tgx_model_desc& d = c->d;
-  if (!c->oproj_sliced || R != 1 || kv_stride == 0 || c->attn_direct || c->attn_mfma || c->gpt2 || c->dt == tgx::DT_F32 || !c->slab_acc) return false;
+  if (c->kv4 || !c->oproj_sliced || R != 1 || kv_stride == 0 || c->attn_direct || c->attn_mfma || c->gpt2 || c->dt == tgx::DT_F32 || !c->slab_acc) return false;
   if (d.head_dim != 64 || d.qk_norm || d.inter > 16384 || c->attn_nsplit > 32) return false;
   if (d.hidden > tgx::XACC_HIDDEN_MAX) return false;     // the fixed-point gate_up hands the converted residual to its waves through hidden * 4 bytes of LDS
   const int qd = d.heads * d.head_dim;
@@ -120,7 +120,7 @@ bool oproj_sliced_ok(const tgx_ctx* c, int R, long long kv_stride) {
 // 600 20.2 / 21.0 / 21.8 -> 18.8 / 19.9 / 21.4 us, Llama-3.2-1B 33.3 / 34.2 / 35.5 -> 30.9 / 32.9 / 34.3; the split form is ahead from ~700 / ~900 keys.
 bool oproj_fused_capable(const tgx_ctx* c) {
   const tgx_model_desc& d = c->d;
-  if (!c->oproj_fused || c->gpt2 || c->dt == tgx::DT_F32 || !c->slab_acc) return false;
+  if (c->kv4 || !c->oproj_fused || c->gpt2 || c->dt == tgx::DT_F32 || !c->slab_acc) return false;
   return d.head_dim == 64 && !d.qk_norm && d.inter <= 16384 && d.hidden % 8 == 0 && d.hidden <= tgx::XACC_HIDDEN_MAX;
 }
 bool oproj_fused_ok(const tgx_ctx* c, int R, long long kv_stride) {
@@ -136,7 +136,7 @@ int launch_layer_kernel(tgx_ctx* c, RowState* rv, int R, int l, int cls, float* 
   RowState& r = rv[0];   // R consecutive row views with the slabs' row strides; kv_stride = 0 when the rows are positions of ONE sequence
   const int H = d.hidden, I = d.inter, hd = d.head_dim, qd = d.heads * hd, kvd = d.kv_heads * hd;
   // bytes between a layer's caches (ebyte pointers): a row's slab [kv_heads][max_ctx][hd], or — paged KV — the layer's pool of KV_BLOCK-token blocks
-  const size_t kv_layer = (c->kv_paged ? (size_t)c->kv_nblocks * d.kv_heads * tgx::KV_BLOCK : (size_t)d.kv_heads * d.max_ctx) * hd * c->esz;
+  const size_t kv_layer = kv_layer_elems(c) * c->esz;
   // paged: the rows share the pools (no row stride) and differ by their block tables; rows that are positions of ONE sequence (kv_stride 0) share one table
   const long long kvs = c->kv_paged ? 0 : kv_stride, tbs = (c->kv_paged && kv_stride != 0) ? c->kv_tbl_stride : 0;
   const LayerW& w = c->L[(size_t)l];
@@ -168,6 +168,7 @@ int launch_layer_kernel(tgx_ctx* c, RowState* rv, int R, int l, int cls, float* 
       break;
     }
     case TGX_KERNEL_ATTN: {  // flashAttention(q, Kall, Vall) over keys [0, pos[row]]; blockIdx.y = batch row (own cache, own length)
+      if (c->kv4) { kv4_step_attend(c, rv, R, l, kv_stride == 0); break; }
       tgx::AttnArgs a{};
       a.q = r.q; a.k_cache = r.kcache + (size_t)l * kv_layer; a.v_cache = r.vcache + (size_t)l * kv_layer;
       a.pos = r.pos; a.part = r.attn_part; a.out = r.attn;

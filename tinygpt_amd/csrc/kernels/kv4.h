@@ -65,18 +65,17 @@ template <bool MAX> __device__ __forceinline__ float kv4_extreme32(float v) {
 // lanes.  A value word holds seven other tokens' codes, which stay: OWNED = nothing else writes the word in this launch, and it is read and stored; otherwise the
 // eight codes of a word may come from several entries and the change goes in by an atomic exclusive or, whose result does not depend on the order.
 template <int HD, bool OWNED>
-__device__ __forceinline__ void kv4_append_one(const Kv4Args& a, unsigned int* page, long long tok, int pos, int kvh) {
+__device__ __forceinline__ void kv4_append_one(const Kv4Args& a, unsigned int* page, int e, long long tok, int pos, int kvh) {
   constexpr int ROUNDS = HD / 64;
   const int lane = threadIdx.x & 63;
   const int t = pos & (KV4_BLK - 1);
   unsigned int* blk = page + (size_t)((pos >> 5) & 3) * kv4_block_words<HD>();
-  const long long slot = (long long)(pos & (KV_BLOCK - 1)) * a.slot_s;
   float x[ROUNDS][2];
 #pragma unroll
   for (int r = 0; r < ROUNDS; r++) {
     const bool val = HD == 64 ? lane >= 32 : r == 1;
     const int ch = HD == 64 ? 2 * (lane & 31) : 2 * lane;
-    const long long at = val ? tok * a.v_ts + kvh * a.v_hs + slot + ch : tok * a.k_ts + kvh * a.k_hs + slot + ch;
+    const long long at = kv4_kv_at(a, e, tok, pos, kvh, val) + ch;
     const void* src = val ? a.v : a.k;
     x[r][0] = kv4_load(src, at, a.kv_dt);
     x[r][1] = kv4_load(src, at + 1, a.kv_dt);
@@ -119,7 +118,7 @@ __global__ __launch_bounds__(64) void kv4_append_token_kernel(const Kv4Args a) {
   const int i = blockIdx.y, pos = en.start + i;
   if (i >= en.count || pos < 0) return;
   unsigned int* page = kv4_page(a, en.seq, pos >> KV4_PAGE_SHIFT, blockIdx.x, HD);
-  if (page) kv4_append_one<HD, false>(a, page, en.tok0 + i, pos, blockIdx.x);
+  if (page) kv4_append_one<HD, false>(a, page, blockIdx.z, en.tok0 + i, pos, blockIdx.x);
 }
 
 // Portions: a workgroup of 2 HD threads a (entry, block of 32 positions, kv head).  Two neighbouring lanes take a group of one token, 32 channels each (32 tokens x HD / 64 groups x {key, value}):
@@ -143,7 +142,7 @@ __global__ __launch_bounds__(2 * HD) void kv4_append_block_kernel(const Kv4Args 
     const bool in = pos >= p0 && pos < p1;
     const int sp = in ? pos : p0;                               // (a lane without a token reads one that is there)
     const long long tok = en.tok0 + sp - en.start;
-    const elem_t<DT>* src = static_cast<const elem_t<DT>*>(val ? a.v : a.k) + (val ? tok * a.v_ts + kvh * a.v_hs : tok * a.k_ts + kvh * a.k_hs) + (long long)(sp & (KV4_PAGE - 1)) * a.slot_s + g * 64 + 32 * half;
+    const elem_t<DT>* src = static_cast<const elem_t<DT>*>(val ? a.v : a.k) + kv4_kv_at(a, blockIdx.z, tok, sp, kvh, val) + g * 64 + 32 * half;
     float x[32];
     if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll
@@ -609,7 +608,7 @@ __device__ __forceinline__ void kv4_append_first(const Kv4Args& a, const Kv4Entr
     const int b = en.start >> KV4_PAGE_SHIFT;
     if (b >= rg.lo && b < rg.hi) {
       unsigned int* page = kv4_page(a, en.seq, b, kvh, HD);
-      if (page && threadIdx.x < 64) kv4_append_one<HD, true>(a, page, en.tok0, en.start, kvh);
+      if (page && threadIdx.x < 64) kv4_append_one<HD, true>(a, page, blockIdx.z, en.tok0, en.start, kvh);
       __syncthreads();
     }
   }

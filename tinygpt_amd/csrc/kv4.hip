@@ -59,7 +59,7 @@ int check_cache(const tgx_kv4_cache* c, const tgx_kv4_batch* b, tgx::Kv4Args& a)
   a.pool = (unsigned int*)c->pool; a.pages = c->pages; a.table = c->table; a.table_stride = c->table_stride; a.table_len = c->table_len; a.seqs = c->seqs;
   a.kv_heads = c->kv_heads;
   a.entries = b->entries; a.max_count = b->offsets ? (int)std::min<int64_t>(b->max_count, b->tokens) : std::min(b->max_count, 1); a.tokens = b->tokens;
-  a.seq = b->seq; a.start = b->start; a.offsets = b->offsets;
+  a.each = 1; a.seq = b->seq; a.start = b->start; a.offsets = b->offsets;
   return TGX_OK;
 }
 
@@ -151,6 +151,155 @@ void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws,
 void launch_copy_pages(const tgx::CopyPagesArgs& a, int layers, hipStream_t s) {
   if (!a.n || !layers || !a.page) return;
   hipLaunchKernelGGL(tgx::copy_pages_kernel, dim3((unsigned)((a.page + tgx::COPY_PIECE - 1) / tgx::COPY_PIECE), a.n, layers), dim3(256), 0, s, a);
+}
+
+// ---- a context's cache in 4 bits (ctx.h) ----------------------------------------------------------------------------------------------------------------
+namespace {
+
+// table of rows whose every entry names one block of their own (steps), or runs of blocks (prompts): row b, entry i -> b * per + min(i, per - 1)
+__global__ __launch_bounds__(256) void stage_tbl_kernel(int* tbl, int stride, int per) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < stride) tbl[(size_t)blockIdx.y * stride + i] = blockIdx.y * per + (i < per ? i : per - 1);
+}
+
+// the pages of layer l through the tables of rows that start at `tbl`
+tgx::Kv4Args layer_args(const tgx_ctx* c, int l, const int* tbl, int rows) {
+  tgx::Kv4Args a{};
+  a.kv_heads = c->d.kv_heads;
+  a.pool = c->kv4_pool + (size_t)l * c->kv_nblocks * tgx::kv4_page_words(a.kv_heads, c->d.head_dim);
+  a.pages = c->kv_nblocks;
+  a.table = tbl; a.table_stride = a.table_len = c->kv_tbl_stride; a.seqs = rows;
+  a.kv_dt = c->dt;
+  return a;
+}
+
+// the workspace of the steps of up to R rows
+size_t step_floats(const tgx_ctx* c) {
+  size_t need = 0;
+  for (int R = 1; R <= std::max(4, c->d.max_batch); R++)
+    for (long long keys = 256;; keys *= 2) {
+      const tgx::Kv4Plan p = tgx::kv4_plan(R, 1, c->d.kv_heads, c->d.heads / c->d.kv_heads, c->d.head_dim, 0, keys, c->num_cus);
+      need = std::max(need, tgx::kv4_part_floats(p, (long long)R * c->d.heads, c->d.head_dim));
+      if (keys >= c->d.max_ctx) break;
+    }
+  return need;
+}
+
+}  // namespace
+
+int kv4_alloc(tgx_ctx* c) {
+  const tgx_model_desc& d = c->d;
+  const size_t B = (size_t)d.max_batch, words = (size_t)d.layers * c->kv_nblocks * tgx::kv4_page_words(d.kv_heads, d.head_dim);
+  int rc;
+  if ((rc = dev_alloc(c, &c->kv4_pool, words))) return rc;
+  HIP_OK(c, hipMemset(c->kv4_pool, 0, words * 4));
+  if ((rc = dev_alloc(c, &c->kv4_stage_tbl, B * (size_t)c->kv_tbl_stride)) || (rc = dev_alloc(c, &c->kv4_prompt_tbl, B * (size_t)c->kv_tbl_stride)) || (rc = dev_alloc(c, &c->kv4_zero, 1))) return rc;
+  HIP_OK(c, hipMemset(c->kv4_zero, 0, 4));
+  hipLaunchKernelGGL(stage_tbl_kernel, dim3((c->kv_tbl_stride + 255) / 256, (unsigned)B), dim3(256), 0, c->stream, c->kv4_stage_tbl, c->kv_tbl_stride, 1);
+  HIP_OK(c, hipGetLastError());
+  c->kv4_ws_floats = step_floats(c);
+  return c->kv4_ws_floats ? dev_alloc(c, &c->kv4_ws, c->kv4_ws_floats) : TGX_OK;
+}
+
+int kv4_prompt_begin(tgx_ctx* c, int row0, int NB, int S) {
+  const size_t per = (size_t)(S + tgx::KV_BLOCK - 1) / tgx::KV_BLOCK, need = per * (size_t)NB, block = (size_t)c->d.kv_heads * tgx::KV_BLOCK * c->d.head_dim * c->esz;
+  if (need > c->kv4_prompt_blocks) {
+    HIP_OK(c, hipStreamSynchronize(c->stream));
+    if (c->kv4_pk) (void)hipFree(c->kv4_pk);
+    if (c->kv4_pv) (void)hipFree(c->kv4_pv);
+    c->kv4_pk = c->kv4_pv = nullptr; c->kv4_prompt_blocks = 0;
+    int rc;
+    if ((rc = dev_alloc(c, &c->kv4_pk, need * block)) || (rc = dev_alloc(c, &c->kv4_pv, need * block))) return rc;
+    c->kv4_prompt_blocks = need;
+    HIP_OK(c, hipMemsetAsync(c->kv4_pk, 0, need * block, c->stream));      // (a tile's tail behind the prompt is read and masked: numbers, as in a cache)
+    HIP_OK(c, hipMemsetAsync(c->kv4_pv, 0, need * block, c->stream));
+  }
+  hipLaunchKernelGGL(stage_tbl_kernel, dim3((c->kv_tbl_stride + 255) / 256, NB), dim3(256), 0, c->stream, c->kv4_prompt_tbl, c->kv_tbl_stride, (int)per);
+  for (int b = 0; b < NB; b++) {
+    RowState& r = c->rows[(size_t)(row0 + b)];
+    r.kcache = c->kv4_pk; r.vcache = c->kv4_pv; r.tbl = c->kv4_prompt_tbl + (size_t)b * c->kv_tbl_stride;
+  }
+  return TGX_OK;
+}
+
+void kv4_prompt_end(tgx_ctx* c, int row0, int NB) {
+  for (int b = row0; b < row0 + NB; b++) {
+    RowState& r = c->rows[(size_t)b];
+    r.kcache = c->slab_k; r.vcache = c->slab_v; r.tbl = c->kv4_stage_tbl + (size_t)b * c->kv_tbl_stride;
+  }
+}
+
+void kv4_prompt_append(tgx_ctx* c, int l, int row0, int NB, int S) {
+  const long long hd = c->d.head_dim, per = (S + tgx::KV_BLOCK - 1) / tgx::KV_BLOCK;
+  tgx::Kv4Args a = layer_args(c, l, c->rows[(size_t)row0].tbl4, NB);
+  a.entries = NB; a.each = a.max_count = S; a.tokens = (long long)NB * S;
+  a.start = c->rows[(size_t)row0].pos;                                  // (0: a prompt's pass moves them when it is through)
+  a.k = c->kv4_pk; a.v = c->kv4_pv;
+  a.k_hs = a.v_hs = tgx::KV_BLOCK * hd; a.slot_s = hd; a.block_s = c->d.kv_heads * tgx::KV_BLOCK * hd; a.entry_s = per * a.block_s;
+  kv4_launch_append(a, (int)hd, c->stream);
+}
+
+// == append and flashAttention over keys [0, pos[row]] of R rows (Attention.h:103-112); one_sequence: the rows are positions of one sequence (a prompt by steps)
+void kv4_step_attend(tgx_ctx* c, RowState* rv, int R, int l, bool one_sequence) {
+  const tgx_model_desc& d = c->d;
+  const long long hd = d.head_dim, qd = (long long)d.heads * hd;
+  RowState& r = rv[0];
+  tgx::Kv4Args a = layer_args(c, l, r.tbl4, R);
+  if (one_sequence) a.table_stride = 0;
+  a.entries = R; a.each = a.max_count = 1; a.tokens = R; a.start = r.pos;
+  // the rows' staging blocks (positions of one sequence: places of one block)
+  const long long block = d.kv_heads * tgx::KV_BLOCK * hd;
+  ebyte *k = r.kcache, *v = r.vcache;
+  if (one_sequence) { const long long row = (r.tbl4 - c->kv_tbl) / c->kv_tbl_stride; k += row * block * c->esz; v += row * block * c->esz; }
+  else { const long long row = rv - c->rows.data(); k += row * block * c->esz; v += row * block * c->esz; }
+  a.k = k; a.v = v; a.k_hs = a.v_hs = tgx::KV_BLOCK * hd; a.slot_s = hd; a.entry_s = one_sequence ? 0 : block;
+  a.q = r.q; a.out = r.attn; a.q_dt = tgx::DT_F32; a.q_ts = a.o_ts = qd; a.q_hs = a.o_hs = hd;
+  a.heads = d.heads; a.group = d.heads / d.kv_heads;
+  tgx::kv4_scale(a, 1.0f / sqrtf((float)hd));
+  a.act16 = c->act16 ? (c->dt == tgx::DT_BF16 ? 1 : 2) : 0;
+  const tgx::Kv4Plan p = tgx::kv4_plan(R, 1, d.kv_heads, a.group, d.head_dim, 0, c->kv4_keys, c->num_cus);
+  if (one_sequence) { kv4_launch_append(a, d.head_dim, c->stream); a.k = a.v = nullptr; }      // (a position reads what the others of the pass append)
+  if (tgx::kv4_part_floats(p, a.tokens * d.heads, d.head_dim) > c->kv4_ws_floats) { c->launch_fault = "kv.bits 4: attention workspace"; return; }
+  kv4_launch_attend(a, p, d.head_dim, c->kv4_ws, c->stream);
+}
+
+static int rows_copy(tgx_ctx* c, int row, int layer, float** tmp, size_t T, tgx::Kv4Args* a) {
+  const size_t n = T * c->d.kv_heads * c->d.head_dim;
+  if (hipMalloc((void**)tmp, 2 * n * 4) != hipSuccess) { (void)hipGetLastError(); return set_err(c, TGX_ERR_NOMEM, "%zu bytes of device memory", 2 * n * 4); }
+  *a = layer_args(c, layer, c->rows[(size_t)row].tbl4, 1);
+  a->entries = 1; a->each = a->max_count = (int)T; a->tokens = (long long)T; a->start = c->kv4_zero;
+  a->k = *tmp; a->v = *tmp + n; a->kv_dt = tgx::DT_F32;
+  a->k_ts = a->v_ts = (long long)c->d.kv_heads * c->d.head_dim; a->k_hs = a->v_hs = c->d.head_dim;
+  return TGX_OK;
+}
+int kv4_read_rows(tgx_ctx* c, int row, int layer, float* k_out, float* v_out, size_t T) {
+  if (!T) return TGX_OK;
+  float* tmp = nullptr;
+  tgx::Kv4Args a{};
+  int rc = rows_copy(c, row, layer, &tmp, T, &a);
+  if (rc) return rc;
+  const size_t n = T * c->d.kv_heads * c->d.head_dim;
+  kv4_launch_read(a, c->d.head_dim, c->stream);
+  if (hipGetLastError() != hipSuccess) rc = set_err(c, TGX_ERR_DEVICE, "kv4 read");
+  if (!rc && k_out) rc = copy_to_host(c, k_out, tmp, n * 4);
+  if (!rc && v_out) rc = copy_to_host(c, v_out, tmp + n, n * 4);
+  (void)hipStreamSynchronize(c->stream);
+  (void)hipFree(tmp);
+  return rc;
+}
+int kv4_write_rows(tgx_ctx* c, int row, int layer, const float* k_in, const float* v_in, size_t T) {
+  if (!T) return TGX_OK;
+  float* tmp = nullptr;
+  tgx::Kv4Args a{};
+  int rc = rows_copy(c, row, layer, &tmp, T, &a);
+  if (rc) return rc;
+  const size_t n = T * c->d.kv_heads * c->d.head_dim;
+  hipError_t e = hipMemcpy(tmp, k_in, n * 4, hipMemcpyHostToDevice);
+  if (e == hipSuccess) e = hipMemcpy(tmp + n, v_in, n * 4, hipMemcpyHostToDevice);
+  if (e == hipSuccess) { kv4_launch_append(a, c->d.head_dim, c->stream); e = hipGetLastError(); }
+  if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+  (void)hipFree(tmp);
+  return e == hipSuccess ? TGX_OK : set_err(c, TGX_ERR_DEVICE, "kv4 write: %s", hipGetErrorString(e));
 }
 
 extern "C" {

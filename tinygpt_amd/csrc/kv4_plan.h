@@ -19,9 +19,11 @@ struct Kv4Args {
   const int* table; int table_stride, table_len, seqs;        // [seqs][table_stride], table_len entries of a row count; a page outside [0, pages) counts as one without tokens
   int kv_heads;
   int entries, max_count; long long tokens;                   // the batch: entries of consecutive tokens of a sequence each
-  const int *seq, *start, *offsets;                           // seq: entry's table row (null: entry e is row e); start: position of its first token; offsets [entries + 1] into the tokens (null: one token each)
-  // keys and values that join (append), or that come out (read): element (token, kv head, channel) at token * k_ts + head * k_hs + (position % KV4_PAGE) * slot_s + channel
-  void *k, *v; int kv_dt; long long k_ts, k_hs, v_ts, v_hs, slot_s;
+  int each;                                                   // tokens of an entry where there are no offsets
+  const int *seq, *start, *offsets;                           // seq: entry's table row (null: entry e is row e); start: position of its first token; offsets [entries + 1] into the tokens (or null)
+  // keys and values that join (append), or that come out (read): (token, kv head, channel) at token * k_ts + head * k_hs + channel elements, and in a context's staging blocks (token strides
+  // of 0) at entry * entry_s + position / KV4_PAGE * block_s + position % KV4_PAGE * slot_s further on
+  void *k, *v; int kv_dt; long long k_ts, k_hs, v_ts, v_hs, slot_s, block_s, entry_s;
   // attention
   const void* q; void* out; int q_dt; long long q_ts, q_hs, o_ts, o_hs;
   int heads, group;
@@ -37,11 +39,16 @@ TGX_KV4 Kv4Entry kv4_entry(const Kv4Args& a, int e) {
   Kv4Entry n;
   n.seq = a.seq ? a.seq[e] : e;
   n.start = a.start[e] < -(1 << 30) ? -(1 << 30) : a.start[e];
-  const long long o0 = a.offsets ? a.offsets[e] : e, c = a.offsets ? a.offsets[e + 1] - o0 : 1;
+  const long long o0 = a.offsets ? a.offsets[e] : (long long)e * a.each, c = a.offsets ? a.offsets[e + 1] - o0 : a.each;
   n.tok0 = o0;
   n.count = (int)(c < a.max_count ? c : a.max_count);
   if (o0 < 0 || c < 0 || o0 + n.count > a.tokens || n.seq < 0 || n.seq >= a.seqs || n.start > 0x7fffffff - n.count) n.count = 0;
   return n;
+}
+
+// elements in front of channel 0 of a key (value) of entry e's token `tok` at `pos`
+TGX_KV4 long long kv4_kv_at(const Kv4Args& a, int e, long long tok, int pos, int kvh, bool value) {
+  return tok * (value ? a.v_ts : a.k_ts) + kvh * (value ? a.v_hs : a.k_hs) + e * a.entry_s + (pos >> KV4_PAGE_SHIFT) * a.block_s + (pos & (KV4_PAGE - 1)) * a.slot_s;
 }
 
 // the words of a page's head, or null where the table names no page

@@ -384,7 +384,7 @@ void launch_embed_rows(tgx_ctx* c, const long long* ids, float* X, int M, int S)
 void launch_prefill(tgx_ctx* c, int row0, int NB, int S, int past) {
   const tgx_model_desc& d = c->d;
   const int H = d.hidden, I = d.inter, hd = d.head_dim, qd = d.heads * hd, kvd = d.kv_heads * hd;
-  const size_t kv_layer = c->kv_paged ? (size_t)c->kv_nblocks * d.kv_heads * tgx::KV_BLOCK * hd : (size_t)d.kv_heads * d.max_ctx * hd;      // elements (paged KV: a layer's pool)
+  const size_t kv_layer = kv_layer_elems(c);
   const int M = NB * S;
   const size_t wout = (size_t)qd + 2 * kvd;
   // GPT-2 (ModelGPT2.h:23-208): wte + wpe rows, LayerNorm with bias ahead of both products, a bias on every Conv1D, c_fc -> gelu_new;
@@ -435,6 +435,7 @@ void launch_prefill(tgx_ctx* c, int row0, int NB, int S, int past) {
       a.scale = 1.0f / sqrtf((float)hd); a.qblk_mirror = 1; a.blk_tbl = r.tbl;
       launch_attn_prefill(c, a, /*allow_lean=*/true);
     }
+    if (c->kv4) kv4_prompt_append(c, l, row0, NB, S);
     int osl = 1;
     launch_gemm(c, tgx::GEMM_RESIDUAL, w.wo, w.bo, c->ws_x, M, H, qd, H, false, nullptr, nullptr, 0, c->gpt2 ? nullptr : &osl);
     if (c->gpt2) {

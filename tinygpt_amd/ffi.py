@@ -87,6 +87,8 @@ ABI = {
     "forward_row": (c_int, [c_void_p, c_int, POINTER(c_int64), c_int]),
     "sample_row": (c_int, [c_void_p, c_int, POINTER(SamplerCfg), c_uint64, POINTER(c_int64)]),
     "past_length_row": (c_int64, [c_void_p, c_int]),
+    "fork_row": (c_int, [c_void_p, c_int, c_int]),
+    "resize_kv": (c_int, [c_void_p, c_int]),
     "context_size": (c_int64, [c_void_p]),
     "num_layers": (c_int32, [c_void_p]),
     "last_error": (c_char_p, [c_void_p]),
@@ -302,6 +304,17 @@ class Model:
         out = c_int64()
         self._check(self.be.sample_row(self._ctx, row, ctypes.byref(cfg), seed, ctypes.byref(out)))
         return out.value
+
+    def fork_row(self, src: int, dst: int):
+        """row `dst` (retired, or the next free one) becomes a copy of live row `src`; paged caches only: whole blocks are shared, the last one is copied"""
+        self._check(self.be.fork_row(self._ctx, src, dst))
+        self.batch = max(self.batch, dst + 1)
+        return self
+
+    def resize_kv(self, budget_tokens: int):
+        """the paged cache's pools made larger or smaller while its rows live"""
+        self._check(self.be.resize_kv(self._ctx, budget_tokens))
+        return self
 
     def past_length_row(self, row: int) -> int:
         return self.be.past_length_row(self._ctx, row)

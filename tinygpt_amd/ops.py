@@ -6,6 +6,8 @@ that grows by concatenation (src/engine/CacheManager.h:24-51) and its attention 
 
 Every call runs on the current stream of the tensors' device and may be captured into a graph: positions, sequences and offsets are read on the device when
 the call runs.  Tensors need no particular strides, only a head's channels lie together.
+
+torch brings a HIP runtime of its own, which the library shares if torch was loaded first: a program that uses both imports torch, or this module, before its first Model.
 """
 from __future__ import annotations
 
@@ -28,11 +30,20 @@ _AT_CACHE, _AT_BATCH, _AT_Q, _AT_K, _AT_V, _AT_OUT = 0, 64, 128, 160, 192, 224
 _local = threading.local()
 
 
+def _one_runtime(maps):
+    """refuses a process (its memory map's lines) that holds two HIP runtimes: neither knows the other's memory and streams"""
+    found = sorted({line.split()[-1] for line in maps if "/libamdhip64.so" in line})
+    if len(found) > 1:
+        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(found)}): import torch or tinygpt_amd.ops before the first Model of the process")
+
+
 class _Calls:
     """the library's entry points, addresses as integers"""
 
     def __init__(self):
         self.be = product_backend()
+        with open("/proc/self/maps") as maps:
+            _one_runtime(maps)
         p, i, q, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
         for name, res, args in (("kv4_append", i, [p] * 4 + [i, p]), ("kv4_read", i, [p] * 4 + [i, p]), ("kv4_attend_workspace", q, [p, p, i, i, q, i]),
                                 ("kv4_attend", i, [p, p, p, i, p, p, f, i, q, p, p, q, i, p]), ("copy_pages", i, [p, q, q, p, q, q, i, q, p, p, i, i, p])):
@@ -213,7 +224,6 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, into: t
 
     pool, into: [layers][pages][...] whose pages lie without gaps, a multiple of 16 bytes each; src, dst: int32.  A pair with a page that does not exist is left out;
     a page that is copied from is not copied to in the same call, and none is copied to twice."""
-    c = _calls()
     n = len(src) if src.dim() == 1 else -1
     sizes = []
     for name, t in (("pool", pool),) if into is None else (("pool", pool), ("into", into)):
@@ -226,5 +236,6 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, into: t
     if into is not None and (a[3:] != b[3:] or pool.device != into.device):
         raise ValueError(f"pools of {a[3]} and {b[3]} layers, pages of {a[4]} and {b[4]} bytes, on {pool.device} and {into.device}")
     dev = pool.device
+    c = _calls()
     c.check(c.copy_pages(*a[:3], *b[:3], a[3], a[4], _int32("src", src, n, dev), _int32("dst", dst, n, dev), n, dev.index, _stream(dev)))
     return pool if into is None else into
