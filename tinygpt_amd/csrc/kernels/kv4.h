@@ -277,6 +277,26 @@ __device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
   return __builtin_bit_cast(bf16x8_t, f);
 }
 constexpr int kv4_slot[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+// 32-bit outputs (TP 3) take the values' codes and levels about their middle, step (n - 7.5) and lo + 7.5 step: values of both signs leave a sum far below that of their codes, whose
+// roundings would stay in it.  And a step's products are summed from zero and join the sums in f32: the matrix unit cuts off what lies below its largest term's last bits.  A window
+// of 4096 keys: 1.8e-6 from the 64-bit sums and 21.8 us without either, 5e-7 and 23.8 us so (plain 32-bit sums of the values: 8e-7); the keys' codes about their middle too, 3e-7 and 25.7 us.
+template <int TP> constexpr bool kv4_about_middle() { return TP == 3; }
+template <int TP> __device__ __forceinline__ bf16x8_t kv4_operand(unsigned int w) {
+  if constexpr (!kv4_about_middle<TP>()) return kv4_frag(w);
+  // a byte of sign and |2 n - 15| is the fp8 number (2 n - 15) / 512; codes below 8 turn round
+  auto centred = [](unsigned int n) {
+    const unsigned int low = ~n & 0x08080808u;
+    return (((n ^ (low - (low >> 3))) & 0x07070707u) << 1) | 0x01010101u | (low << 4);
+  };
+  const unsigned int a = centred(w & 0x0f0f0f0fu), b = centred((w >> 4) & 0x0f0f0f0fu);
+  u32x4 f;
+  f[0] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 256.f, false));
+  f[1] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 256.f, true));
+  f[2] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 256.f, false));
+  f[3] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 256.f, true));
+  return __builtin_bit_cast(bf16x8_t, f);
+}
+template <int TP> __device__ __forceinline__ float kv4_base(float lo, float step) { return kv4_about_middle<TP>() ? fmaf(7.5f, step, lo) : lo; }
 // over the lanes of equal r: lanes 16 and 32 further swap in the vector registers
 __device__ __forceinline__ float kv4_max_quarters(float v) {
   u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
@@ -289,6 +309,13 @@ __device__ __forceinline__ float kv4_sum_quarters(float v) {
   v = __uint_as_float(w[0]) + __uint_as_float(w[1]);
   w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
   return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+// what weights of an old reference (a score) are of a new one.  Weights are 2^(score scale - reference scale) with the second product rounded: the factor is made of the rounded ones, or
+// sums of different references would be off by their difference.  Records of sums hold the rounded product.
+__device__ __forceinline__ float kv4_factor(float was, float is, float scale) {
+#pragma clang fp contract(off)
+  const float a = was * scale, b = is * scale;
+  return __builtin_amdgcn_exp2f(a - b);
 }
 // the page of a block, -1: none.  Tables are read through the scalar cache: an entry in front of its use costs no vector register and waits for no vector load
 __device__ __forceinline__ int kv4_page_id(const Kv4Args& a, int seq, int b, int b_hi) {
@@ -362,7 +389,7 @@ struct Kv4Sums {
   float qsum[NT][G];
   int pos[NT];                                                // a column's position; -1: no column
   f32x4 o[NT][CT];
-  float m[NT], l[NT], lov[NT][G];                             // m: the reference of the weights, in scores before the scale
+  float m[NT], l[NT], lov[NT][G];                             // m: the reference of the weights, in scores before the scale (records hold it behind it)
 
   __device__ __forceinline__ void start(const Kv4Args& a, const Kv4Entry& en, int kvh, int col0, int ncol, int q4, int r16) {
 #pragma unroll
@@ -459,7 +486,7 @@ struct Kv4Sums {
       mx = kv4_max_quarters(mx);
       // the sums keep their reference until a maximum passes it by 8 in the exponent (weights up to 256 then): few blocks rescale
       if (__any(mx > m[t] + gap)) {
-        const float nm = fmaxf(m[t], mx), f = nm > m[t] ? __builtin_amdgcn_exp2f((m[t] - nm) * scale) : 1.f;
+        const float nm = fmaxf(m[t], mx), f = nm > m[t] ? kv4_factor(m[t], nm, scale) : 1.f;
         m[t] = nm;
         l[t] *= f;
 #pragma unroll
@@ -495,7 +522,7 @@ struct Kv4Sums {
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const unsigned int w = par[i][r][g];
-            const float st = bf16_hi(w), lo = bf16_lo(w);
+            const float st = bf16_hi(w), lo = kv4_base<TP>(bf16_lo(w), st);
             ps[4 * i + r] = MASK && !seen[t][i][r] ? 0.f : p[t][i][r] * st;
             lov[t][g] = MASK && !seen[t][i][r] ? lov[t][g] : fmaf(p[t][i][r], lo, lov[t][g]);
           }
@@ -510,11 +537,15 @@ struct Kv4Sums {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const int x = 4 * g + c;
-        const bf16x8_t vf = kv4_frag(raw.v[x >> 2][x & 3]);
+        const bf16x8_t vf = kv4_operand<TP>(raw.v[x >> 2][x & 3]);
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NT; t++) {
+          f32x4 sum = kv4_about_middle<TP>() ? f32x4{0.f, 0.f, 0.f, 0.f} : o[t][x];
 #pragma unroll
-          for (int term = 0; term < TP; term++) o[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][term]), vf, o[t][x], 0, 0, 0);
+          for (int term = TP - 1; term >= 0; term--) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pf[t][term]), vf, sum, 0, 0, 0);
+          if constexpr (kv4_about_middle<TP>()) o[t][x] += sum;
+          else o[t][x] = sum;
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -581,7 +612,7 @@ __device__ __forceinline__ void kv4_meet(const Kv4Args& a, const Kv4Entry& en, i
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < KW; w++) {
-      const float mw = s_ml[w][c][0], f = mw == mx ? 1.f : __builtin_amdgcn_exp2f((mw - mx) * a.scale_log2);      // (all -inf: sums of zero)
+      const float mw = s_ml[w][c][0], f = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);      // (all -inf: sums of zero)
       const f32x4 v = *reinterpret_cast<const f32x4*>(so + (w * nv + c) * HD + 4 * x);
       den = fmaf(f, s_ml[w][c][1], den);
 #pragma unroll
@@ -641,7 +672,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
     const int c0 = col0 + 16 * t, nv = min(16, ncol - c0);
     if (nv <= 0) break;
     if (t > 0) __syncthreads();
-    if (q4 == 0) { s_ml[wv][r16][0] = s.m[t]; s_ml[wv][r16][1] = s.l[t]; }
+    if (q4 == 0) { s_ml[wv][r16][0] = s.m[t] * a.scale_log2; s_ml[wv][r16][1] = s.l[t]; }
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const int c = 4 * q4 + r;
@@ -678,7 +709,7 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
     const int mine = col0 + 16 * t + r16;
     if (a.splits > 1 && mine < ncol && q4 == 0) {
       const long long rec = ((en.tok0 + mine / a.group) * a.heads + kvh * a.group + mine % a.group) * a.splits + split;
-      a.ml[rec * 2] = s.m[t];
+      a.ml[rec * 2] = s.m[t] * a.scale_log2;
       a.ml[rec * 2 + 1] = s.l[t];
     }
 #pragma unroll
@@ -846,7 +877,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
           w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false));
           mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
         }
-        const float f = mx > m[r] ? __builtin_amdgcn_exp2f((m[r] - mx) * scale) : 1.f;
+        const float f = mx > m[r] ? kv4_factor(m[r], mx, scale) : 1.f;
         m[r] = mx; ref[r] = -mx * scale;
         l[r] *= f;
 #pragma unroll
@@ -866,7 +897,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
     for (int g = 0; g < G; g++) {
       float ps[4];
 #pragma unroll
-      for (int r = 0; r < 4; r++) { ps[r] = p[r] * st[1][g]; lov[g][r] = fmaf(p[r], lo[1][g], lov[g][r]); }
+      for (int r = 0; r < 4; r++) { ps[r] = p[r] * st[1][g]; lov[g][r] = fmaf(p[r], kv4_base<TP>(lo[1][g], st[1][g]), lov[g][r]); }
 #pragma unroll
       for (int term = 0; term < TP; term++) {
 #pragma unroll
@@ -884,19 +915,27 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 #pragma unroll
         for (int term = 0; term < TP; term++) wf[x][term] = *reinterpret_cast<const bf16x8_t*>(&s_w[wv][term][n16 % RPT][32 * x + 8 * q4]);
       wave_fence();
+      f32x4 sum[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) sum[c] = kv4_about_middle<TP>() ? f32x4{0.f, 0.f, 0.f, 0.f} : o[4 * g + c];
 #pragma unroll
       for (int x = 0; x < NB; x++) {
         bf16x8_t vf[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           const int i = 4 * g + c;
-          vf[c] = kv4_frag(rv[x][i >> 2][i & 3]);
-          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][0], vf[c], o[i], 0, 0, 0);
+          vf[c] = kv4_operand<TP>(rv[x][i >> 2][i & 3]);
+          sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][TP - 1], vf[c], sum[c], 0, 0, 0);
         }
 #pragma unroll
-        for (int term = 1; term < TP; term++)
+        for (int term = TP - 2; term >= 0; term--)
 #pragma unroll
-          for (int c = 0; c < 4; c++) o[4 * g + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], vf[c], o[4 * g + c], 0, 0, 0);
+          for (int c = 0; c < 4; c++) sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[x][term], vf[c], sum[c], 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        if constexpr (kv4_about_middle<TP>()) o[4 * g + c] += sum[c];
+        else o[4 * g + c] = sum[c];
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -927,7 +966,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
     for (int r = 0; r < 4; r++) {
       const int c = 4 * q4 + r;
       if (c < nv) {
-        if (n16 == 0) { s_ml[wv][c][0] = m[r]; s_ml[wv][c][1] = l[r]; }
+        if (n16 == 0) { s_ml[wv][c][0] = -ref[r]; s_ml[wv][c][1] = l[r]; }
 #pragma unroll
         for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + n16] = o[x][r];
       }
@@ -955,7 +994,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
     mx = group_max<64>(mx);
     float tot = 0.f;
     for (int s = tid; s < S; s += 64) {
-      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f((ms - mx) * a.scale_log2);
+      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f(ms - mx);
       sw[s] = w;
       tot += w * ml[2 * s + 1];
     }
