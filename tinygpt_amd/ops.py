@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import struct
 import threading
 
@@ -24,7 +25,7 @@ PAGE_TOKENS = 128
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 # A call's structs (include/tgx.h) are packed into one buffer of the calling thread, at fixed places, and go to the library as addresses: a few calls of a step are short
-# enough for their binding to count (an attention call: 22 us with a ctypes object a struct, 11 so, of which the library and its two launches take most).
+# enough for their binding to count (an attention call: 22 us with a ctypes object a struct, 8 so, of which the library and its launches take half).
 _CACHE, _BATCH, _ROWS = struct.Struct("QqQ5i4x"), struct.Struct("2iq3Q"), struct.Struct("Qi4x2q")
 _AT_CACHE, _AT_BATCH, _AT_Q, _AT_K, _AT_V, _AT_OUT = 0, 64, 128, 160, 192, 224
 _local = threading.local()
@@ -93,17 +94,17 @@ class Kv4Cache:
     def __init__(self, pool: torch.Tensor, table: torch.Tensor, kv_heads: int, head_dim: int):
         if head_dim not in (64, 128) or kv_heads < 1:
             raise ValueError(f"a 4-bit cache of {kv_heads} heads of {head_dim} channels is not built (head_dim 64 and 128 are)")
-        nbytes, shape = kv_heads * head_dim * 144, pool.shape
-        if len(shape) < 3 or not pool.is_contiguous() or shape[2:].numel() * pool.element_size() != nbytes:
+        nbytes, shape, device = kv_heads * head_dim * 144, pool.shape, pool.device
+        if len(shape) < 3 or not pool.is_contiguous() or math.prod(shape[2:]) * pool.element_size() != nbytes:
             raise ValueError(f"pool: contiguous [layers][pages][...] with {nbytes} bytes a page")
-        if table.dtype != torch.int32 or table.dim() != 2:
+        if table.dtype is not torch.int32 or table.dim() != 2:
             raise ValueError("table: int32 [sequences][pages of one]")
         (seqs, length), (stride, one) = table.shape, table.stride()
         if length > 1 and one != 1 or seqs > 1 and stride < length:
             raise ValueError("table: a sequence's entries lie together and are its own")
-        if not pool.is_cuda or pool.device != table.device:
-            raise ValueError(f"pool ({pool.device}) and table ({table.device}) are on one GPU")
-        self.pool, self.table, self.kv_heads, self.head_dim, self.device, self.layers = pool, table, kv_heads, head_dim, pool.device, shape[0]
+        if device.type != "cuda" or device != table.device:
+            raise ValueError(f"pool ({device}) and table ({table.device}) are on one GPU")
+        self.pool, self.table, self.kv_heads, self.head_dim, self.device, self.index, self.layers = pool, table, kv_heads, head_dim, device, device.index, shape[0]
         self._at, self._layer_bytes = pool.data_ptr(), shape[1] * nbytes
         self._rest = (shape[1], table.data_ptr(), stride if seqs > 1 else length, length, seqs, kv_heads, head_dim)
 
@@ -120,7 +121,7 @@ class Kv4Cache:
 
 
 def _int32(name, t, n, device):
-    if t.dtype != torch.int32 or t.shape != (n,) or n > 1 and t.stride(0) != 1 or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name}: int32 [{n}] without gaps on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -153,8 +154,7 @@ def _pack_rows(buf, at, name, t, tokens, heads, cache):
     _ROWS.pack_into(buf, at, t.data_ptr(), dtype, token, head)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_stream = torch._C._cuda_getCurrentRawStream      # of a device's index; as torch.cuda.current_stream(device).cuda_stream, without the object around it (0.1 us for 1.9)
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, layer: int = 0, seq: torch.Tensor = None, offsets: torch.Tensor = None,
@@ -169,7 +169,7 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
     _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
     _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
     cache._pack(buf, layer)
-    c.check(c.kv4_append(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.device.index, _stream(cache.device)))
+    c.check(c.kv4_append(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.index, _stream(cache.index)))
 
 
 def kv4_read(cache: Kv4Cache, start: torch.Tensor, tokens: int, dtype: torch.dtype = torch.float32, layer: int = 0, seq: torch.Tensor = None, offsets: torch.Tensor = None,
@@ -182,7 +182,7 @@ def kv4_read(cache: Kv4Cache, start: torch.Tensor, tokens: int, dtype: torch.dty
     _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
     _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
     cache._pack(buf, layer)
-    c.check(c.kv4_read(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.device.index, _stream(cache.device)))
+    c.check(c.kv4_read(at + _AT_CACHE, at + _AT_BATCH, at + _AT_K, at + _AT_V, cache.index, _stream(cache.index)))
     return k, v
 
 
@@ -201,7 +201,7 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
     entries, max_count = _pack_batch(buf, cache, tokens, start, seq, offsets, max_count)
     _pack_rows(buf, _AT_Q, "q", q, tokens, heads, cache)
     if out is None:
-        out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype:
         raise ValueError(f"out: {q.dtype} as q, got {out.dtype}")
     _pack_rows(buf, _AT_OUT, "out", out, tokens, heads, cache)
@@ -211,11 +211,11 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
         _pack_rows(buf, _AT_K, "k", k, tokens, cache.kv_heads, cache)
         _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
     cache._pack(buf, layer)
-    index = cache.device.index
+    index = cache.index
     need = _workspace(entries, max_count, tokens, cache.kv_heads, cache.head_dim, heads, window, max_keys, index)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     c.check(c.kv4_attend(at + _AT_CACHE, at + _AT_BATCH, at + _AT_Q, heads, None if k is None else at + _AT_K, None if k is None else at + _AT_V, cache.head_dim ** -0.5 if scale is None else scale,
-                         window, max_keys, at + _AT_OUT, ws.data_ptr() if need else None, need, index, _stream(cache.device)))
+                         window, max_keys, at + _AT_OUT, ws.data_ptr() if need else None, need, index, _stream(index)))
     return out
 
 
@@ -237,5 +237,5 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, into: t
         raise ValueError(f"pools of {a[3]} and {b[3]} layers, pages of {a[4]} and {b[4]} bytes, on {pool.device} and {into.device}")
     dev = pool.device
     c = _calls()
-    c.check(c.copy_pages(*a[:3], *b[:3], a[3], a[4], _int32("src", src, n, dev), _int32("dst", dst, n, dev), n, dev.index, _stream(dev)))
+    c.check(c.copy_pages(*a[:3], *b[:3], a[3], a[4], _int32("src", src, n, dev), _int32("dst", dst, n, dev), n, dev.index, _stream(dev.index)))
     return pool if into is None else into
