@@ -454,6 +454,25 @@ def test_streams_and_graphs(torch):
         torch.randn(1 << 20, device="cuda").sum()
 
 
+@pytest.mark.parametrize("offsets", [False, True])
+@pytest.mark.parametrize("heads,n", [(2, 700), (8, 90), (32, 300)])
+def test_entries_of_one_sequence_see_each_other(torch, heads, n, offsets):
+    """the last tokens of a sequence as entries of one token each, in any order: as appended first, bit for bit"""
+    new = 9
+    rows = [Rows(torch, [n], 2, 64, "bf16", room=new).fill() for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(new, heads, 64, device="cuda", generator=g).bfloat16()
+    order = [4, 8, 0, 7, 3, 1, 6, 2, 5]
+    k = torch.stack([rows[0].k[n + i] for i in order])
+    v = torch.stack([rows[0].v[n + i] for i in order])
+    batch = dict(seq=ints(torch, [0] * new), offsets=ints(torch, range(new + 1)) if offsets else None, max_count=1 if offsets else None)
+    start = ints(torch, [n + i for i in order])
+    out = rows[0].ops.kv4_attend(rows[0].cache, q, start, n + new, k=k, v=v, **batch)
+    rows[1].ops.kv4_append(rows[1].cache, k, v, start, **batch)
+    want = rows[1].ops.kv4_attend(rows[1].cache, q, start, n + new, **batch)
+    assert torch.equal(out, want) and torch.equal(rows[0].cache.pool, rows[1].cache.pool)
+
+
 def test_same_call_same_bits(torch):
     r = Rows(torch, [5000, 60], 4, 128, "bf16").fill()
     q = torch.randn(2, 16, 128, device="cuda").bfloat16()
@@ -476,3 +495,15 @@ def test_refused_tensors(torch):
         with pytest.raises(TgxError):
             ops.kv4_attend(c, *args, **more)
     assert ops.kv4_attend(c, q[:0], s[:0], 10).shape == (0, 8, 64)
+
+
+def test_tensors_that_ask_for_gradients_are_refused(torch):
+    r = Rows(torch, [5], 1, 64, "bf16", room=1).fill()
+    start = ints(torch, [4])
+    q = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        r.ops.kv4_attend(r.cache, q, start, 5)
+    with pytest.raises(ValueError, match="gradient"):
+        r.ops.kv4_append(r.cache, r.k[5:].clone().requires_grad_(), r.v[5:], start)
+    with torch.no_grad():
+        assert not r.ops.kv4_attend(r.cache, q, start, 5).requires_grad

@@ -123,10 +123,11 @@ static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStrea
   else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TP>), grid, dim3(256), 0, s, a);
 }
 
-// a.splits, a.part, a.ml follow from the plan and the workspace here; with keys and values to append that the attention launch does not append itself, an append launch first
+// a.splits, a.part, a.ml follow from the plan and the workspace here.  Keys and values to append: a single token's join in the attention launch, where an entry is its sequence's only one
+// (3 us less than a launch of its own); entries that name their sequences or bring several tokens may read what others bring, and an append launch comes first
 void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws, hipStream_t s) {
   if (!a.entries || !a.max_count) return;
-  if (a.k && a.max_count > 1) { kv4_launch_append(a, hd, s); a.k = a.v = nullptr; }
+  if (a.k && (a.max_count > 1 || a.seq || a.offsets)) { kv4_launch_append(a, hd, s); a.k = a.v = nullptr; }
   const size_t rows = (size_t)a.tokens * a.heads;
   a.splits = p.splits;
   a.part = ws; a.ml = ws + rows * p.splits * hd;

@@ -5,7 +5,8 @@ on a GPU.  Format, page layout and what happens to pages that a table does not n
 that grows by concatenation (src/engine/CacheManager.h:24-51) and its attention is one library call over it (src/layer/Attention.h:103-112).
 
 Every call runs on the current stream of the tensors' device and may be captured into a graph: positions, sequences and offsets are read on the device when
-the call runs.  Tensors need no particular strides, only a head's channels lie together.
+the call runs.  Tensors need no particular strides, only a head's channels lie together.  There are no gradients: tensors that ask
+for one are refused.
 
 torch brings a HIP runtime of its own, which the library shares if torch was loaded first: a program that uses both imports torch, or this module, before its first Model.
 """
@@ -148,6 +149,8 @@ def _pack_rows(buf, at, name, t, tokens, heads, cache):
         raise ValueError(f"{name}: bfloat16, float16 or float32, got {t.dtype}")
     if t.device != cache.device:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and a 4-bit cache has none: torch.no_grad() or detach()")
     token, head, channel = t.stride()
     if channel != 1:
         raise ValueError(f"{name}: a head's channels lie together (stride 1)")
