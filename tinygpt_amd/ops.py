@@ -194,7 +194,7 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
     """Attention of queries [tokens][heads][head_dim] over the cache (== flashAttention over what the reference's cache returns).
 
     The batch's tokens are named as in kv4_append; a token at position p sees its sequence's keys at 0 .. p, with window > 0 the last `window` of them.  k, v: the tokens'
-    own keys and values, which join the cache first (then a token sees itself); without them they are there already.  max_keys: at least the last position + 1 of every
+    own keys and values, which join the cache first (a token sees itself, and what other entries bring in front of it in its sequence); without them they are there already.  max_keys: at least the last position + 1 of every
     entry, to divide the work by.  scale: head_dim ** -0.5 where not given.  A token that sees nothing gets zeros; one that no entry names stays as it was in `out` (in a
     new one it holds anything)."""
     c, (buf, at) = _calls(), _buffer()
