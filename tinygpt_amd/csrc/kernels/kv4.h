@@ -263,8 +263,8 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
 // them) meet the codes, the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A
 // operand of P V, whose contraction runs over the tokens in the order of the value words.
 // TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17) leave an output
-// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, took a portion of 2048 tokens from 672 us to 573 and left it 1.55 times as far from
-// 64 bits: its rounding meets the levels' spread.)
+// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, takes a portion of 2048 tokens from 587 us to 497
+// with the values about the middle of their levels, and one long row from 38.4 to 35.3; outputs are 1.4 times as far from 64 bits then.)
 // A word's codes as bf16 numbers, exactly: a byte n of 0 .. 15 is the fp8 (e4m3) number n / 512, and the conversion scales.  They come in the order e = 0, 4, 1, 5, 2, 6, 3, 7, in which
 // what they are multiplied with is laid out (kv4_slot: the code at a place).
 __device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
@@ -386,7 +386,11 @@ template <int HD, int NT, int TQ, int TP>
 struct Kv4Sums {
   static constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16;
   bf16x8_t qf[NT][CH][TQ];
-  float qsum[NT][G];
+  // The sums of a query's channels of a group, which meet the los: in f32, or for queries of one term (whose operands leave the registers) as three terms (2^-25) of a product of its own, at
+  // places 3 g .. 3 g + 2 of quarter 0
+  static constexpr bool LO_PRODUCT = TQ == 1;
+  float qsum[NT][LO_PRODUCT ? 1 : G];
+  bf16x8_t qlo[LO_PRODUCT ? NT : 1];
   int pos[NT];                                                // a column's position; -1: no column
   f32x4 o[NT][CT];
   float m[NT], l[NT], lov[NT][G];                             // m: the reference of the weights, in scores before the scale (records hold it behind it)
@@ -399,7 +403,8 @@ struct Kv4Sums {
       const long long base = (en.tok0 + i) * a.q_ts + h * a.q_hs + 8 * q4;
       m[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; g++) { qsum[t][g] = 0.f; lov[t][g] = 0.f; }
+      for (int g = 0; g < G; g++) lov[t][g] = 0.f;
+      float sum[G] = {};
 #pragma unroll
       for (int x = 0; x < CT; x++) o[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -414,49 +419,83 @@ struct Kv4Sums {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             f[e] = pack_bf16(x[kv4_slot[2 * e]], x[kv4_slot[2 * e + 1]]);
-            qsum[t][ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
+            sum[ch / 2] += bf16_lo(f[e]) + bf16_hi(f[e]);
             x[kv4_slot[2 * e]] -= bf16_lo(f[e]); x[kv4_slot[2 * e + 1]] -= bf16_hi(f[e]);
           }
           qf[t][ch][term] = __builtin_bit_cast(bf16x8_t, f);
         }
       }
 #pragma unroll
-      for (int g = 0; g < G; g++) qsum[t][g] = kv4_sum_quarters(qsum[t][g]);
+      for (int g = 0; g < G; g++) sum[g] = kv4_sum_quarters(sum[g]);
+      if constexpr (LO_PRODUCT) {
+        u32x4 f = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+          for (int i = 3 * g; i < 3 * g + 3; i++) {
+            const unsigned int term = pack_bf16(sum[g], 0.f) & 0xffffu;
+            sum[g] -= bf16_lo(term);
+            f[i >> 1] |= q4 == 0 ? term << (16 * (i & 1)) : 0u;
+          }
+        qlo[t] = __builtin_bit_cast(bf16x8_t, f);
+      } else {
+#pragma unroll
+        for (int g = 0; g < G; g++) qsum[t][g] = sum[g];
+      }
     }
   }
 
   // One block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters, which every lane needs of the four tokens of its scores.  MASK: some column does not
   // see some token of the block; what is not seen is selected away, whatever it holds.  In phases that the compiler does not mix: mixed, their registers are half again as many.
   template <bool MASK>
-  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, unsigned int* sp, int lane) {
+  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, float* sp, int lane) {
     const int q4 = lane >> 4;
-    constexpr int PW = HD / 32;                               // parameter words of a token: keys, then values
-    if constexpr (PW == 4) *reinterpret_cast<u32x4*>(sp + (lane & 31) * 4) = u32x4{raw.p[0], raw.p[1], raw.p[2], raw.p[3]};
-    else *reinterpret_cast<u32x2*>(sp + (lane & 31) * 2) = u32x2{raw.p[0], raw.p[1]};
+    // Each token's levels become numbers once: floats [step of the keys' groups, lo of them, step of the values', base of them][32 tokens]; lanes of 32 and beyond take the values'
+    {
+      const bool values = lane >= 32;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const unsigned int w = values ? raw.p[G + g] : raw.p[g];
+        const float st = bf16_hi(w), lo = bf16_lo(w);
+        float* to = sp + (values ? 64 * G : 0) + (lane & 31);
+        to[32 * g] = st;
+        to[32 * (G + g)] = values ? kv4_base<TP>(lo, st) : lo;
+      }
+    }
     wave_fence();
-    // the keys' (which 0) or the values' (1) parameters of a lane's tokens
-    auto parameters = [&](unsigned int (&par)[2][4][G], int which) {
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int g = 0; g < G; g++) par[i][r][g] = sp[(16 * i + 4 * q4 + r) * PW + which * G + g];
+    // the steps and los (bases) of a lane's four tokens of tile i: keys (0) or values (1)
+    auto levels = [&](int which, int i, int g, f32x4& st, f32x4& lo) {
+      st = *reinterpret_cast<const f32x4*>(sp + (which * 2 * G + g) * 32 + 16 * i + 4 * q4);
+      lo = *reinterpret_cast<const f32x4*>(sp + (which * 2 * G + G + g) * 32 + 16 * i + 4 * q4);
     };
-    unsigned int par[2][4][G];
-    parameters(par, 0);
+    // the los of tile i's tokens as a row's operand: a token's lo at its group's three places, the same in every quarter (a product with zeros keeps a token's NaN to the token)
+    bf16x8_t lof[2];
+    if constexpr (LO_PRODUCT) {
+      u32x2 w[G];
+#pragma unroll
+      for (int g = 0; g < G; g++) w[g] = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(raw.p[g], raw.p[g], false, false));
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const unsigned int a = __builtin_amdgcn_perm(w[0][i], w[0][i], 0x01000100u), b = __builtin_amdgcn_perm(w[G - 1][i], w[0][i], 0x05040100u);
+        const unsigned int c = __builtin_amdgcn_perm(w[G - 1][i], w[G - 1][i], 0x01000100u);
+        lof[i] = __builtin_bit_cast(bf16x8_t, u32x4{a, b, c, c});
+      }
+    }
     f32x4 sc[NT][2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (LO_PRODUCT) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lof[i], qlo[t], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      }
 #pragma unroll
       for (int g = 0; g < G; g++) {
         bf16x8_t kf[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(raw.k[x >> 2][x & 3]); }
-        float st[4], z[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) { st[r] = bf16_hi(par[i][r][g]); z[r] = bf16_lo(par[i][r][g]); }
+        f32x4 st, z;
+        levels(0, i, g, st, z);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -465,7 +504,7 @@ struct Kv4Sums {
 #pragma unroll
             for (int term = 0; term < TQ; term++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], qf[t][2 * g + c][term], d, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; r++) sc[t][i][r] = fmaf(st[r], d[r], g == 0 ? z[r] * qsum[t][g] : fmaf(z[r], qsum[t][g], sc[t][i][r]));
+          for (int r = 0; r < 4; r++) sc[t][i][r] = fmaf(st[r], d[r], LO_PRODUCT ? sc[t][i][r] : g == 0 ? z[r] * qsum[t][g] : fmaf(z[r], qsum[t][g], sc[t][i][r]));
         }
       }
     }
@@ -509,10 +548,11 @@ struct Kv4Sums {
         }
     }
     __builtin_amdgcn_sched_barrier(0);
-    parameters(par, 1);
-    wave_fence();
 #pragma unroll
     for (int g = 0; g < G; g++) {
+      f32x4 vst[2], vlo[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) levels(1, i, g, vst[i], vlo[i]);
       u32x4 pf[NT][TP];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -521,10 +561,8 @@ struct Kv4Sums {
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const unsigned int w = par[i][r][g];
-            const float st = bf16_hi(w), lo = kv4_base<TP>(bf16_lo(w), st);
-            ps[4 * i + r] = MASK && !seen[t][i][r] ? 0.f : p[t][i][r] * st;
-            lov[t][g] = MASK && !seen[t][i][r] ? lov[t][g] : fmaf(p[t][i][r], lo, lov[t][g]);
+            ps[4 * i + r] = MASK && !seen[t][i][r] ? 0.f : p[t][i][r] * vst[i][r];
+            lov[t][g] = MASK && !seen[t][i][r] ? lov[t][g] : fmaf(p[t][i][r], vlo[i][r], lov[t][g]);
           }
 #pragma unroll
         for (int term = 0; term < TP; term++)
@@ -549,12 +587,13 @@ struct Kv4Sums {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    wave_fence();
   }
 
   // The blocks b0, b0 + STEP, .. below b1, every one (MASK false) or only those of them outside of [skip0, skip1) (MASK true): one on its way while one is worked on, the page of the one behind on its way
   // before that.  A walk takes one kind of block: with both in one loop the compiler keeps two sets of sums.
   template <bool MASK, int STEP>
-  __device__ __forceinline__ void walk(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, unsigned int* sp, int lane) {
+  __device__ __forceinline__ void walk(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, float* sp, int lane) {
     const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
     const size_t page_words = (size_t)a.kv_heads * (36 * HD);
     auto past = [&](int b) { return MASK && b >= skip0 && b < skip1 ? b + (skip1 - b + STEP - 1) / STEP * STEP : b; };
@@ -570,7 +609,7 @@ struct Kv4Sums {
   }
   // a wave's blocks (b_lo + first, in steps) of columns at positions p0 .. p1: those that every column sees whole, then the others
   template <int STEP>
-  __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, unsigned int* sp, int lane) {
+  __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, float* sp, int lane) {
     // whole for every column: t0 + 31 <= p0 and t0 > p1 - window
     int w1 = (p0 + 1) >> 5, w0 = a.window > 0 && p1 - a.window + 1 > 0 ? (p1 - a.window + KV4_BLK) >> 5 : 0;
     w1 = min(max(w1, 0), b_hi);
@@ -651,7 +690,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
   extern __shared__ __attribute__((aligned(16))) float kv4_lds[];
-  __shared__ __attribute__((aligned(16))) unsigned int s_par[KW][HD];
+  __shared__ __attribute__((aligned(16))) float s_par[KW][2 * HD];
   __shared__ float s_ml[KW][16][2];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
@@ -690,7 +729,7 @@ template <int HD, int NT, int TQ, int TP>
 __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
-  __shared__ __attribute__((aligned(16))) unsigned int s_par[4][HD];
+  __shared__ __attribute__((aligned(16))) float s_par[4][2 * HD];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
