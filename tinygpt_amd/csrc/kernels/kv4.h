@@ -447,15 +447,16 @@ struct Kv4Sums {
 
   // One block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters, which every lane needs of the four tokens of its scores.  MASK: some column does not
   // see some token of the block; what is not seen is selected away, whatever it holds.  In phases that the compiler does not mix: mixed, their registers are half again as many.
-  template <bool MASK>
-  __device__ __forceinline__ void block(const Kv4Raw<HD>& raw, int t0, int window, float scale, float gap, float* sp, int lane) {
+  // key, value: the block's operands, by their number.
+  template <bool MASK, typename Keys, typename Values>
+  __device__ __forceinline__ void block(const Keys& key, const Values& value, const unsigned int (&par)[HD / 32], int t0, int window, float scale, float gap, float* sp, int lane) {
     const int q4 = lane >> 4;
     // Each token's levels become numbers once: floats [step of the keys' groups, lo of them, step of the values', base of them][32 tokens]; lanes of 32 and beyond take the values'
     {
       const bool values = lane >= 32;
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const unsigned int w = values ? raw.p[G + g] : raw.p[g];
+        const unsigned int w = values ? par[G + g] : par[g];
         const float st = bf16_hi(w), lo = bf16_lo(w);
         float* to = sp + (values ? 64 * G : 0) + (lane & 31);
         to[32 * g] = st;
@@ -473,7 +474,7 @@ struct Kv4Sums {
     if constexpr (LO_PRODUCT) {
       u32x2 w[G];
 #pragma unroll
-      for (int g = 0; g < G; g++) w[g] = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(raw.p[g], raw.p[g], false, false));
+      for (int g = 0; g < G; g++) w[g] = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(par[g], par[g], false, false));
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const unsigned int a = __builtin_amdgcn_perm(w[0][i], w[0][i], 0x01000100u), b = __builtin_amdgcn_perm(w[G - 1][i], w[0][i], 0x05040100u);
@@ -493,7 +494,7 @@ struct Kv4Sums {
       for (int g = 0; g < G; g++) {
         bf16x8_t kf[2];
 #pragma unroll
-        for (int c = 0; c < 2; c++) { const int x = i * CH + 2 * g + c; kf[c] = kv4_frag(raw.k[x >> 2][x & 3]); }
+        for (int c = 0; c < 2; c++) kf[c] = key(i * CH + 2 * g + c);
         f32x4 st, z;
         levels(0, i, g, st, z);
 #pragma unroll
@@ -575,7 +576,7 @@ struct Kv4Sums {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const int x = 4 * g + c;
-        const bf16x8_t vf = kv4_operand<TP>(raw.v[x >> 2][x & 3]);
+        const bf16x8_t vf = value(x);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           f32x4 sum = kv4_about_middle<TP>() ? f32x4{0.f, 0.f, 0.f, 0.f} : o[t][x];
@@ -603,21 +604,73 @@ struct Kv4Sums {
     while (b < b1) {
       const int bm = past(bn + STEP), idm = kv4_page_id(a, seq, bm, b1);
       if (idn >= 0) nxt.load(heads + idn * page_words + (size_t)(bn & 3) * kv4_block_words<HD>(), lane);
-      if (id >= 0) block<MASK>(raw, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
+      if (id >= 0)
+        block<MASK>([&](int x) { return kv4_frag(raw.k[x >> 2][x & 3]); }, [&](int x) { return kv4_operand<TP>(raw.v[x >> 2][x & 3]); }, raw.p, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
       raw = nxt; b = bn; id = idn; bn = bm; idn = idm;
     }
+  }
+  // the blocks [w0, w1) that columns at positions p0 .. p1 all see whole: t0 + 31 <= p0 and t0 > p1 - window
+  static __device__ __forceinline__ void whole(const Kv4Args& a, int b_hi, int p0, int p1, int& w0, int& w1) {
+    w1 = min(max((p0 + 1) >> 5, 0), b_hi);
+    w0 = min(a.window > 0 && p1 - a.window + 1 > 0 ? (p1 - a.window + KV4_BLK) >> 5 : 0, w1);
   }
   // a wave's blocks (b_lo + first, in steps) of columns at positions p0 .. p1: those that every column sees whole, then the others
   template <int STEP>
   __device__ __forceinline__ void all(const Kv4Args& a, int seq, int kvh, int first_block, int b_hi, int p0, int p1, float* sp, int lane) {
-    // whole for every column: t0 + 31 <= p0 and t0 > p1 - window
-    int w1 = (p0 + 1) >> 5, w0 = a.window > 0 && p1 - a.window + 1 > 0 ? (p1 - a.window + KV4_BLK) >> 5 : 0;
-    w1 = min(max(w1, 0), b_hi);
-    w0 = min(w0, w1);
+    int w0, w1;
+    whole(a, b_hi, p0, p1, w0, w1);
     int f = first_block;
     if (f < w0) f += (w0 - f + STEP - 1) / STEP * STEP;
     walk<false, STEP>(a, seq, kvh, f, w1, 0, 0, sp, lane);
     walk<true, STEP>(a, seq, kvh, first_block, b_hi, w0, w1, sp, lane);
+  }
+
+  // A workgroup's walk, four waves on the same blocks: a wave makes a quarter of a block's operands, all read them from LDS ([2][key operands, value operands][64] of them), which takes
+  // three quarters of the conversions away.  Every wave comes here with the same blocks; mine: this wave has columns that see something up to position `until`.
+  template <bool MASK>
+  __device__ __forceinline__ void walk_shared(const Kv4Args& a, int seq, int kvh, int b0, int b1, int skip0, int skip1, bool mine, int until, bf16x8_t* so, float* sp, int wv, int lane) {
+    constexpr int P = HD / 64, ONE = 2 * CT * 64;              // operands of a wave and kind, of a block
+    const unsigned int* heads = a.pool + (size_t)kvh * (36 * HD);
+    const size_t page_words = (size_t)a.kv_heads * (36 * HD);
+    auto past = [&](int b) { return MASK && b >= skip0 && b < skip1 ? skip1 : b; };
+    unsigned int k[P] = {}, v[P] = {}, par[HD / 32] = {}, par_next[HD / 32] = {};
+    auto load = [&](int id, int b) {
+      const unsigned int* blk = heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>();
+      const int x = wv * P, at = ((x >> 2) * 64 + lane) * 4 + (x & 3);
+      if constexpr (P == 2) {
+        const u32x2 kk = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(blk + at)), vv = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(blk + 4 * HD + at));
+        k[0] = kk[0]; k[1] = kk[1]; v[0] = vv[0]; v[1] = vv[1];
+        const u32x4 w = load_nt(reinterpret_cast<const u32x4*>(blk + 8 * HD) + (lane & 31));
+        par_next[0] = w[0]; par_next[1] = w[1]; par_next[2] = w[2]; par_next[3] = w[3];
+      } else {
+        k[0] = __builtin_nontemporal_load(blk + at); v[0] = __builtin_nontemporal_load(blk + 4 * HD + at);
+        const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(blk + 8 * HD) + (lane & 31));
+        par_next[0] = w[0]; par_next[1] = w[1];
+      }
+    };
+    auto make = [&](bf16x8_t* to) {
+#pragma unroll
+      for (int i = 0; i < P; i++) { to[(wv * P + i) * 64 + lane] = kv4_frag(k[i]); to[(CT + wv * P + i) * 64 + lane] = kv4_operand<TP>(v[i]); }
+#pragma unroll
+      for (int i = 0; i < HD / 32; i++) par[i] = par_next[i];
+    };
+    int b = past(b0), id = kv4_page_id(a, seq, b, b1), cur = 0;
+    if (b >= b1) return;
+    if (id >= 0) { load(id, b); make(so); }
+    int bn = past(b + 1), idn = kv4_page_id(a, seq, bn, b1);
+    if (idn >= 0) load(idn, bn);
+    __syncthreads();
+    while (b < b1) {
+      const int bm = past(bn + 1), idm = kv4_page_id(a, seq, bm, b1);
+      const bf16x8_t* from = so + cur * ONE + lane;
+      if (id >= 0 && mine && (!MASK || b * KV4_BLK <= until))
+        block<MASK>([&](int x) { return from[x * 64]; }, [&](int x) { return from[(CT + x) * 64]; }, par, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
+      cur ^= 1;
+      if (idn >= 0) make(so + cur * ONE);
+      if (idm >= 0) load(idm, bm);
+      __syncthreads();
+      b = bn; id = idn; bn = bm; idn = idm;
+    }
   }
 
   // o becomes the columns' sums, l their denominators (over the four quarters)
@@ -724,24 +777,29 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   }
 }
 
-// Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys.
+// Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys, whose operands they make together.
 template <int HD, int NT, int TQ, int TP>
 __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
   __shared__ __attribute__((aligned(16))) float s_par[4][2 * HD];
+  __shared__ bf16x8_t s_op[2 * 2 * CT * 64];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
-  const int ncol = en.count * a.group, col0 = ((int)blockIdx.y * 4 + wv) * 16 * NT;
-  if (col0 >= ncol) return;      // (no barrier follows)
-  const int first = en.start + col0 / a.group, last = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;
+  const int ncol = en.count * a.group, wg0 = (int)blockIdx.y * 64 * NT, col0 = wg0 + wv * 16 * NT;
+  if (wg0 >= ncol) return;       // (the whole workgroup)
+  const int first = en.start + wg0 / a.group, last = en.start + min(wg0 + 64 * NT - 1, ncol - 1) / a.group;
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
   const int key_lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   const int b_hi = min(rg.hi * 4, (last >> 5) + 1), b_lo = max(rg.lo * 4, key_lo >> 5);
   Sums s;
   s.start(a, en, kvh, col0, ncol, q4, r16);
-  s.template all<1>(a, en.seq, kvh, b_lo, b_hi, first, last, s_par[wv], lane);
+  const int until = en.start + min(col0 + 16 * NT - 1, ncol - 1) / a.group;
+  int w0, w1;
+  Sums::whole(a, b_hi, first, last, w0, w1);
+  s.template walk_shared<false>(a, en.seq, kvh, max(b_lo, w0), w1, 0, 0, col0 < ncol, until, s_op, s_par[wv], wv, lane);
+  s.template walk_shared<true>(a, en.seq, kvh, b_lo, b_hi, w0, w1, col0 < ncol, until, s_op, s_par[wv], wv, lane);
   s.finish(q4);
 #pragma unroll
   for (int t = 0; t < NT; t++) {
