@@ -787,7 +787,9 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r16 = lane & 15;
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
-  const int ncol = en.count * a.group, wg0 = (int)blockIdx.y * 64 * NT, col0 = wg0 + wv * 16 * NT;
+  // the tiles with most keys first, downwards, then those with fewest, upwards: two workgroups of a compute unit have about the same to do in sum
+  const int tiles = gridDim.y, upper = (tiles + 1) / 2, tile = (int)blockIdx.y < upper ? tiles - 1 - (int)blockIdx.y : (int)blockIdx.y - upper;
+  const int ncol = en.count * a.group, wg0 = tile * 64 * NT, col0 = wg0 + wv * 16 * NT;
   if (wg0 >= ncol) return;       // (the whole workgroup)
   const int first = en.start + wg0 / a.group, last = en.start + min(wg0 + 64 * NT - 1, ncol - 1) / a.group;
   const Kv4Range rg = kv4_range(first, last, a.window, a.table_len, split, a.splits);
