@@ -1075,52 +1075,72 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   kv4_meet<HD, KW, kv4_type<TQ>()>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
 }
 
-// The splits' records of a row (token, query head): a workgroup a row.
+// The splits' records of a row (token, query head): a workgroup a row.  A chain of round trips and no more than that: sums are asked for before the weights are known, and every wave works
+// out all weights (lane s the splits s, s + 64, ..), which go to their sums by lane exchange.
 template <int HD, int DT>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
-  constexpr int LN = HD / 4, WAYS = 256 / LN;                 // lanes of a row, splits at a time
-  __shared__ float sw[1024];
+  constexpr int LN = HD / 4, WAYS = 256 / LN, PER = 64 / WAYS;      // lanes of a row, splits at a time, rounds of 64 splits
   __shared__ f32x4 sacc[256];
-  __shared__ float stot;
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
   if ((int)blockIdx.y >= en.count) return;
-  const int h = blockIdx.x, S = a.splits, tid = threadIdx.x;
+  const int h = blockIdx.x, S = a.splits, tid = threadIdx.x, lane = tid & 63, ln = tid % LN, way = tid / LN;
   const long long row = (en.tok0 + blockIdx.y) * a.heads + h;
   const float* ml = a.ml + row * S * 2;
-  if (tid < 64) {
-    float mx = -INFINITY;
-    for (int s = tid; s < S; s += 64) mx = fmaxf(mx, ml[2 * s]);
-    mx = group_max<64>(mx);
-    float tot = 0.f;
-    for (int s = tid; s < S; s += 64) {
-      const float ms = ml[2 * s], w = ms == mx ? 1.f : __builtin_amdgcn_exp2f(ms - mx);
-      sw[s] = w;
-      tot += w * ml[2 * s + 1];
-    }
-    tot = group_sum<64>(tot);
-    if (tid == 0) stot = tot;
-  }
-  __syncthreads();
-  const int ln = tid % LN, way = tid / LN;
-  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = way; s < S; s += WAYS) {
-    const f32x4 v = reinterpret_cast<const f32x4*>(a.part + (row * S + s) * HD)[ln];
-    const float w = sw[s];
+  const f32x4* part = reinterpret_cast<const f32x4*>(a.part + row * S * HD) + ln;
+  f32x4 v[PER];
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = fmaf(w, v[i], acc[i]);
+  for (int i = 0; i < PER; i++) {
+    const int s = way + i * WAYS;
+    v[i] = s < S ? part[(size_t)s * LN] : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float w[4], l[4], mx = -INFINITY, tot = 0.f;                       // (at most 256 splits)
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    const int s = lane + 64 * q;
+    w[q] = s < S ? ml[2 * s] : -INFINITY;
+    l[q] = s < S ? ml[2 * s + 1] : 0.f;
+    mx = fmaxf(mx, w[q]);
+  }
+  mx = fmaxf(mx, dpp_mov<0xB1, 0xf>(mx));
+  mx = fmaxf(mx, dpp_mov<0x4E, 0xf>(mx));
+  mx = fmaxf(mx, dpp_mov<0x141, 0xf>(mx));
+  mx = fmaxf(mx, dpp_mov<0x140, 0xf>(mx));
+  mx = kv4_max_quarters(mx);
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    w[q] = w[q] == mx ? 1.f : __builtin_amdgcn_exp2f(w[q] - mx);
+    tot = fmaf(w[q], l[q], tot);
+  }
+  tot = kv4_sum_quarters(row_group_sum<16>(tot));
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    if (64 * q >= S) break;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int s = 64 * q + way + i * WAYS;
+      if (q > 0) v[i] = s < S ? part[(size_t)s * LN] : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const float f = __shfl(w[q], way + i * WAYS, 64);
+#pragma unroll
+      for (int c = 0; c < 4; c++) acc[c] = fmaf(f, v[i][c], acc[c]);
+    }
   }
   sacc[tid] = acc;
   __syncthreads();
   if (tid < LN) {
-    for (int w = 1; w < WAYS; w++) {
-      const f32x4 v = sacc[w * LN + tid];
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[i] += v[i];
+    for (int k = 1; k < WAYS; k++) {
+      const f32x4 o = sacc[k * LN + tid];
+#pragma unroll
+      for (int c = 0; c < 4; c++) acc[c] += o[c];
     }
-    const float inv = stot == 0.f ? 0.f : 1.f / stot;
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
     const long long at = (en.tok0 + blockIdx.y) * a.o_ts + h * a.o_hs + 4 * tid;
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] *= inv;
+    for (int c = 0; c < 4; c++) acc[c] *= inv;
     kv4_store4<DT>(a.out, at, acc, a.act16);
   }
 }
