@@ -275,6 +275,27 @@ def test_pages_that_are_not_there_are_not_seen(torch):
         assert (np.abs(out - want) <= bound(want, s, o, 400, EPS["fp32"], 2)).all()
 
 
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("hd,group,gone", [(64, 4, [0]), (128, 4, [1, 2]), (64, 1, [3]), (128, 7, [0, 2, 3]), (64, 16, [0, 1, 2, 3])])
+def test_portions_over_pages_that_are_not_there(torch, hd, group, gone, window):
+    """tokens -7 .. 429 of a sequence some of whose pages are missing, several workgroups of columns"""
+    n, before = 430, 7
+    r = Rows(torch, [n], 2, hd, "fp32", seed=hd + group).fill()
+    r.cache.table[0, gone] = -1
+    q = torch.tensor(np.random.default_rng(4).normal(size=(n + before, 2 * group, hd)), dtype=torch.float32).cuda()
+    out = numpy_of(r.ops.kv4_attend(r.cache, q, ints(torch, [-before]), n, offsets=ints(torch, [0, n + before]), window=window)).astype(np.float64)
+    (k, kb), (v, vb) = r.held(0)
+    there = np.array([p for p in range(n) if p // PAGE not in gone], int)
+    for t in list(range(before)) + [before + p for p in (0, 1, 31, 32, 127, 128, 200, 255, 256, 300, 383, 384, 429)]:
+        pos = t - before
+        keep = there[(there <= pos) & ((window == 0) | (there > pos - window))]
+        if not len(keep):
+            assert not out[t].any()
+            continue
+        want, s, o = attend(numpy_of(q[t:t + 1]), k[keep], v[keep], [len(keep) - 1], big=(kb[keep], vb[keep]))
+        assert (np.abs(out[t:t + 1] - want) <= bound(want, s, o, n, EPS["fp32"], 2)).all(), t
+
+
 def test_positions_behind_the_table_see_its_pages(torch):
     r = Rows(torch, [256], 1, 64, "bf16").fill()
     q = torch.randn(1, 4, 64, device="cuda").bfloat16()

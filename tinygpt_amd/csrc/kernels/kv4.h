@@ -203,7 +203,8 @@ __global__ __launch_bounds__(2 * HD) void kv4_append_block_kernel(const Kv4Args 
   }
 }
 
-// The values that the pages hold for the batch's tokens: a wave a (entry, block of 32 positions, kv head).
+// The values that the pages hold for the batch's tokens: a wave a (entry, block of 32 positions, kv head).  Bound by its stores, 16 bits or more for 4.5 that it reads: four rows of up to 4096
+// tokens, eight heads of 128, 14 us (3.4 TB/s); a token of each of 64 rows 4.2 us.
 template <int HD, int DT>
 __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
   constexpr int PARTS = HD / 64;
@@ -263,8 +264,8 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
 // them) meet the codes, the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A
 // operand of P V, whose contraction runs over the tokens in the order of the value words.
 // TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17) leave an output
-// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, takes a portion of 2048 tokens from 587 us to 497
-// with the values about the middle of their levels, and one long row from 38.4 to 35.3; outputs are 1.4 times as far from 64 bits then.)
+// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, with the values about
+// the middle of their levels: portions in 15 % less time, one long row in 8 %, and outputs 1.4 times as far from 64 bits.)
 // A word's codes as bf16 numbers, exactly: a byte n of 0 .. 15 is the fp8 (e4m3) number n / 512, and the conversion scales.  They come in the order e = 0, 4, 1, 5, 2, 6, 3, 7, in which
 // what they are multiplied with is laid out (kv4_slot: the code at a place).
 __device__ __forceinline__ bf16x8_t kv4_frag(unsigned int w) {
@@ -738,6 +739,7 @@ __device__ __forceinline__ void kv4_append_first(const Kv4Args& a, const Kv4Entr
 }
 
 // Few columns (a few tokens' query heads): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
+// 16 rows of up to 2000 tokens, five tokens each, 16 / 8 heads of 128: 14 us (1.7 TB/s), a way of eight blocks a wave between its start and the meeting of the waves.
 template <int HD, int NT, int KW, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
@@ -777,7 +779,9 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
   }
 }
 
-// Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys, whose operands they make together.
+// Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys, whose operands they make together.  Bound by the vector units, some 370 instructions a
+// block of 32 tokens and 32 columns beside 52 of the matrix units: 2048 tokens behind 6144, 32 / 8 heads of 128, 476 us (505 TFLOP/s).  Operands made by each wave for itself: 30 us more;
+// tiles in their order, so that a compute unit gets two with many keys: 80 us more.
 template <int HD, int NT, int TQ, int TP>
 __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, TQ, TP> Sums;
@@ -835,6 +839,8 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
 // over, so that the products of 16 / RPT tiles of tokens give every lane the scores of one token for four heads (quarter q takes its rows from the product of tile q, or q / 2): a lane
 // reads the parameters of its own token, and each score, exponential and weight is worked out once and not for 16 columns of which RPT are asked for.  The weights
 // pass through LDS into the A operand of P V (rows heads).  What a row's four heads share (references, their sums' factors) is the same in every lane that holds the row.
+// Memory and vector units overlap but for a fifth: 32 rows of up to 4096 tokens, 32 / 8 heads of 128, 24.8 us (4.1 TB/s; 19 to 21 without the arithmetic), one of 131071 with 64 / 8 heads 33.5
+// (4.5 TB/s; 25).  Short rows are one dependent way, table, page, sums: 300 tokens, 7.5 us (3.7 without the arithmetic).
 template <int HD, int RPT, int KW, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args a) {
   constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64, PW = HD / 32;
@@ -1077,6 +1083,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 
 // The splits' records of a row (token, query head): a workgroup a row.  A chain of round trips and no more than that: sums are asked for before the weights are known, and every wave works
 // out all weights (lane s the splits s, s + 64, ..), which go to their sums by lane exchange.
+// 4.0 us behind an attention launch; with weights first, by way of LDS, 4.7.
 template <int HD, int DT>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(const Kv4Args a) {
   constexpr int LN = HD / 4, WAYS = 256 / LN, PER = 64 / WAYS;      // lanes of a row, splits at a time, rounds of 64 splits
@@ -1152,7 +1159,7 @@ struct CopyPagesArgs {
   long long src_pages, dst_pages;                             // pages of a pool
   const int *from, *to; int n;                                // pairs; one outside of its pool is left out
 };
-// a workgroup a (16 KB piece of a page, pair, layer)
+// a workgroup a (16 KB piece of a page, pair, layer): memory's rate, 180 pages of 147 KB in 32 layers 317 us (5.4 TB/s, reads and writes; a copy of 1 GiB has 5.0); a page in 16 layers 3.4 us
 constexpr int COPY_PIECE = 16384;
 static __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyPagesArgs a) {
   const int pair = blockIdx.y;
