@@ -263,8 +263,8 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
 // entry, query head of the kv head) costs two fused multiply-adds a score and group and no value is worked out.  O = P V the same way: the weights p step_g (bf16, TP terms of
 // them) meet the codes, the lo part is summed in f32.  Lane (q, r) holds the scores of column r, tokens 4 q .. 4 q + 3 of a 16-token tile: as it needs them as the A
 // operand of P V, whose contraction runs over the tokens in the order of the value words.
-// TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17) leave an output
-// in 16 bits what its own rounding leaves, three one in 32.  (One, as coarse as an output in bf16, with the values about
+// QT: a query's and an output's type.  TQ, TP: 16-bit terms of a query and of a weight.  Queries in bf16 are one term exactly, in fp16 two, in fp32 three (2^-25).  Of a weight, two (2^-17)
+// leave an output in 16 bits what its own rounding leaves, three one in 32.  A model's steps take its 32-bit activations as two terms (2^-17), as its products do.  (One, as coarse as an output in bf16, with the values about
 // the middle of their levels: portions in 15 % less time, one long row in 8 %, and outputs 1.4 times as far from 64 bits.)
 // A word's codes as bf16 numbers, exactly: a byte n of 0 .. 15 is the fp8 (e4m3) number n / 512, and the conversion scales.  They come in the order e = 0, 4, 1, 5, 2, 6, 3, 7, in which
 // what they are multiplied with is laid out (kv4_slot: the code at a place).
@@ -325,8 +325,6 @@ __device__ __forceinline__ int kv4_page_id(const Kv4Args& a, int seq, int b, int
   const int p = *(const __attribute__((address_space(4))) int*)at;
   return p >= 0 && p < a.pages ? p : -1;
 }
-// a query's and an output's type by the terms of a query
-template <int TQ> constexpr int kv4_type() { return TQ == 1 ? DT_BF16 : TQ == 2 ? DT_F16 : DT_F32; }
 // eight neighbouring channels of a row
 template <int DT>
 __device__ __forceinline__ void kv4_load8(const void* p, long long i, float x[8]) {
@@ -383,7 +381,7 @@ template <int HD> struct Kv4Raw {
 };
 
 // The sums of NT tiles of 16 query columns over the blocks that a wave walks.
-template <int HD, int NT, int TQ, int TP>
+template <int HD, int NT, int QT, int TQ, int TP>
 struct Kv4Sums {
   static constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16;
   bf16x8_t qf[NT][CH][TQ];
@@ -411,7 +409,7 @@ struct Kv4Sums {
 #pragma unroll
       for (int ch = 0; ch < CH; ch++) {
         float x[8];
-        kv4_load8<kv4_type<TQ>()>(a.q, base + 32 * ch, x);
+        kv4_load8<QT>(a.q, base + 32 * ch, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
 #pragma unroll
@@ -740,9 +738,9 @@ __device__ __forceinline__ void kv4_append_first(const Kv4Args& a, const Kv4Entr
 
 // Few columns (a few tokens' query heads): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
 // 16 rows of up to 2000 tokens, five tokens each, 16 / 8 heads of 128: 14 us (1.7 TB/s), a way of eight blocks a wave between its start and the meeting of the waves.
-template <int HD, int NT, int KW, int TQ, int TP>
+template <int HD, int NT, int KW, int QT, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args a) {
-  typedef Kv4Sums<HD, NT, TQ, TP> Sums;
+  typedef Kv4Sums<HD, NT, QT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
   extern __shared__ __attribute__((aligned(16))) float kv4_lds[];
   __shared__ __attribute__((aligned(16))) float s_par[KW][2 * HD];
@@ -775,16 +773,16 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
         for (int x = 0; x < CT; x++) kv4_lds[(wv * nv + c) * HD + 16 * x + r16] = s.o[t][x][r];
     }
     __syncthreads();
-    kv4_meet<HD, KW, kv4_type<TQ>()>(a, en, kvh, split, c0, nv, kv4_lds, s_ml);
+    kv4_meet<HD, KW, QT>(a, en, kvh, split, c0, nv, kv4_lds, s_ml);
   }
 }
 
 // Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys, whose operands they make together.  Bound by the vector units, some 370 instructions a
 // block of 32 tokens and 32 columns beside 52 of the matrix units: 2048 tokens behind 6144, 32 / 8 heads of 128, 476 us (505 TFLOP/s).  Operands made by each wave for itself: 30 us more;
 // tiles in their order, so that a compute unit gets two with many keys: 80 us more.
-template <int HD, int NT, int TQ, int TP>
+template <int HD, int NT, int QT, int TQ, int TP>
 __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
-  typedef Kv4Sums<HD, NT, TQ, TP> Sums;
+  typedef Kv4Sums<HD, NT, QT, TQ, TP> Sums;
   constexpr int CT = Sums::CT;
   __shared__ __attribute__((aligned(16))) float s_par[4][2 * HD];
   __shared__ bf16x8_t s_op[2 * 2 * CT * 64];
@@ -829,7 +827,7 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
         const float inv = den == 0.f ? 0.f : 1.f / den;
         const long long at = (en.tok0 + i) * a.o_ts + h * a.o_hs;
 #pragma unroll
-        for (int x = 0; x < CT; x++) kv4_store1<kv4_type<TQ>()>(a.out, at + 16 * x + r16, s.o[t][x][r] * inv, a.act16);
+        for (int x = 0; x < CT; x++) kv4_store1<QT>(a.out, at + 16 * x + r16, s.o[t][x][r] * inv, a.act16);
       }
     }
   }
@@ -841,7 +839,7 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
 // pass through LDS into the A operand of P V (rows heads).  What a row's four heads share (references, their sums' factors) is the same in every lane that holds the row.
 // Memory and vector units overlap but for a fifth: 32 rows of up to 4096 tokens, 32 / 8 heads of 128, 24.8 us (4.1 TB/s; 19 to 21 without the arithmetic), one of 131071 with 64 / 8 heads 33.5
 // (4.5 TB/s; 25).  Short rows are one dependent way, table, page, sums: 300 tokens, 7.5 us (3.7 without the arithmetic).
-template <int HD, int RPT, int KW, int TQ, int TP>
+template <int HD, int RPT, int KW, int QT, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args a) {
   constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64, PW = HD / 32;
   constexpr int NJ = 16 / RPT, TOK = 16 * NJ, NB = TOK / 32;      // tiles, tokens and blocks of a step
@@ -895,7 +893,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
 #pragma unroll
     for (int ch = 0; ch < CH; ch++) {
       float x[8];
-      kv4_load8<kv4_type<TQ>()>(a.q, base + 32 * ch, x);
+      kv4_load8<QT>(a.q, base + 32 * ch, x);
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] *= a.q_sign;
 #pragma unroll
@@ -1078,7 +1076,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
     }
   }
   __syncthreads();
-  kv4_meet<HD, KW, kv4_type<TQ>()>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
+  kv4_meet<HD, KW, QT>(a, en, kvh, split, 0, nv, kv4_lds, s_ml);
 }
 
 // The splits' records of a row (token, query head): a workgroup a row.  A chain of round trips and no more than that: sums are asked for before the weights are known, and every wave works

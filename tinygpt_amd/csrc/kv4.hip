@@ -107,20 +107,22 @@ void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s) {
     else hipLaunchKernelGGL((tgx::kv4_read_kernel<128, DT>), grid, dim3(64), 0, s, a);)
 }
 
-template <int HD, int TQ, int TP>
+// STEPS: single tokens of a model's rows, and nothing else
+template <int HD, int QT, int TQ, int TP, bool STEPS>
 static void launch_attend(const tgx::Kv4Args& a, const tgx::Kv4Plan& p, hipStream_t s) {
   const dim3 grid(a.kv_heads * p.splits, p.tiles, a.entries);
   const size_t lds = (size_t)p.kw * std::min<long long>(16, (long long)a.max_count * a.group) * HD * 4;
   if (a.max_count == 1 && a.group <= 4) {
-    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 8, TQ, TP>), grid, dim3(512), lds, s, a);
-    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 8, QT, TQ, TP>), grid, dim3(512), lds, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 4, 4, QT, TQ, TP>), grid, dim3(256), lds, s, a);
   } else if (a.max_count == 1 && a.group <= 8) {
-    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 8, TQ, TP>), grid, dim3(512), lds, s, a);
-    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 4, TQ, TP>), grid, dim3(256), lds, s, a);
+    if (p.kw == 8) hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 8, QT, TQ, TP>), grid, dim3(512), lds, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_attend_token_kernel<HD, 8, 4, QT, TQ, TP>), grid, dim3(256), lds, s, a);
+  } else if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, QT, TQ, TP>), grid, dim3(256), lds, s, a);
+  else if constexpr (!STEPS) {
+    if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, QT, TQ, TP>), grid, dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, QT, TQ, TP>), grid, dim3(256), 0, s, a);
   }
-  else if (p.kw == 4 && p.nt == 1) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 1, 4, TQ, TP>), grid, dim3(256), lds, s, a);
-  else if (p.kw == 4) hipLaunchKernelGGL((tgx::kv4_attend_keys_kernel<HD, 2, 4, TQ, TP>), grid, dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((tgx::kv4_attend_columns_kernel<HD, 2, TQ, TP>), grid, dim3(256), 0, s, a);
 }
 
 // a.splits, a.part, a.ml follow from the plan and the workspace here.  Keys and values to append: a single token's join in the attention launch, where an entry is its sequence's only one
@@ -132,15 +134,15 @@ void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws,
   a.splits = p.splits;
   a.part = ws; a.ml = ws + rows * p.splits * hd;
   // terms of queries and weights by the outputs' type (kernels/kv4.h)
-  if (hd == 64) {
-    if (a.q_dt == tgx::DT_BF16) launch_attend<64, 1, 2>(a, p, s);
-    else if (a.q_dt == tgx::DT_F16) launch_attend<64, 2, 2>(a, p, s);
-    else launch_attend<64, 3, 3>(a, p, s);
-  } else {
-    if (a.q_dt == tgx::DT_BF16) launch_attend<128, 1, 2>(a, p, s);
-    else if (a.q_dt == tgx::DT_F16) launch_attend<128, 2, 2>(a, p, s);
-    else launch_attend<128, 3, 3>(a, p, s);
-  }
+  auto launch = [&](auto hd_c) {
+    constexpr int HD = decltype(hd_c)::value;
+    if (a.q_dt == tgx::DT_BF16) launch_attend<HD, tgx::DT_BF16, 1, 2, false>(a, p, s);
+    else if (a.q_dt == tgx::DT_F16) launch_attend<HD, tgx::DT_F16, 2, 2, false>(a, p, s);
+    else if (a.steps && a.max_count == 1) launch_attend<HD, tgx::DT_F32, 2, 2, true>(a, p, s);
+    else launch_attend<HD, tgx::DT_F32, 3, 3, false>(a, p, s);
+  };
+  if (hd == 64) launch(std::integral_constant<int, 64>{});
+  else launch(std::integral_constant<int, 128>{});
   if (p.splits > 1) {
     const dim3 grid(a.heads, a.max_count, a.entries);
     TGX_DT_SWITCH(a.q_dt,
@@ -248,6 +250,7 @@ void kv4_step_attend(tgx_ctx* c, RowState* rv, int R, int l, bool one_sequence) 
   tgx::Kv4Args a = layer_args(c, l, r.tbl4, R);
   if (one_sequence) a.table_stride = 0;
   a.entries = R; a.each = a.max_count = 1; a.tokens = R; a.start = r.pos;
+  a.steps = 1;
   // the rows' staging blocks (positions of one sequence: places of one block)
   const long long block = d.kv_heads * tgx::KV_BLOCK * hd;
   ebyte *k = r.kcache, *v = r.vcache;

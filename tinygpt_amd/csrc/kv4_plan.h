@@ -30,6 +30,7 @@ struct Kv4Args {
   float scale_log2, q_sign, gap;                              // |score scale| * log2(e) (1 for a scale of 0), the scale's sign, 8 / scale_log2: see kv4_scale
   int window;                                                 // > 0: position p sees keys p - window + 1 .. p
   int splits; float *part, *ml;                               // splits > 1: [token * heads + head][splits][HD] sums, [..][splits][2] (maximum, denominator)
+  int steps;                                                  // a model's steps (host only): 32-bit queries in two terms
   int act16;                                                  // outputs rounded to the storage type: 0 no, 1 bf16, 2 fp16 (option act.round16 of a model)
 };
 
