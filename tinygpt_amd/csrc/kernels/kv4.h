@@ -297,6 +297,11 @@ template <int TP> __device__ __forceinline__ bf16x8_t kv4_operand(unsigned int w
   f[3] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 256.f, true));
   return __builtin_bit_cast(bf16x8_t, f);
 }
+// Outputs in 16 bits (TP 2) keep the codes as they are, and a walk's products stay in the matrix unit's sums.  Those are of one sign and grow with the keys while the values' own sum does not: a
+// sum's roundings, 2^-24 of it each, come to more than an output's own rounding over some 10^4 keys (1024 tokens in fp16 behind 32768: 4.4e-4 from 64 bits, behind 131072 1.6e-3; the rounding
+// 2.1e-4).  So the part of the los, of the other sign, joins them every KV4_FOLD blocks, which leaves the values' sum:
+// 8e-6 of a row beside its output's rounding at any length, which is what two terms of a weight leave, for 2 % of a portion's time (476 us: 486) and 1 of one long row's.
+constexpr int KV4_FOLD = 16;
 template <int TP> __device__ __forceinline__ float kv4_base(float lo, float step) { return kv4_about_middle<TP>() ? fmaf(7.5f, step, lo) : lo; }
 // over the lanes of equal r: lanes 16 and 32 further swap in the vector registers
 __device__ __forceinline__ float kv4_max_quarters(float v) {
@@ -442,6 +447,23 @@ struct Kv4Sums {
         for (int g = 0; g < G; g++) qsum[t][g] = sum[g];
       }
     }
+  }
+
+  // the part of the los joins o
+  __device__ __forceinline__ void fold(int q4) {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const float lg = kv4_sum_quarters(lov[t][g]);
+        lov[t][g] = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float add = __shfl(lg, 4 * q4 + r, 64);
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
+        }
+      }
   }
 
   // One block of 32 tokens from position t0 on.  sp: the wave's LDS for the parameters, which every lane needs of the four tokens of its scores.  MASK: some column does not
@@ -599,12 +621,14 @@ struct Kv4Sums {
     auto past = [&](int b) { return MASK && b >= skip0 && b < skip1 ? b + (skip1 - b + STEP - 1) / STEP * STEP : b; };
     Kv4Raw<HD> raw, nxt;
     int b = past(b0), bn = past(b + STEP), id = kv4_page_id(a, seq, b, b1), idn = kv4_page_id(a, seq, bn, b1);
+    int walked = 0;
     if (id >= 0) raw.load(heads + id * page_words + (size_t)(b & 3) * kv4_block_words<HD>(), lane);
     while (b < b1) {
       const int bm = past(bn + STEP), idm = kv4_page_id(a, seq, bm, b1);
       if (idn >= 0) nxt.load(heads + idn * page_words + (size_t)(bn & 3) * kv4_block_words<HD>(), lane);
       if (id >= 0)
         block<MASK>([&](int x) { return kv4_frag(raw.k[x >> 2][x & 3]); }, [&](int x) { return kv4_operand<TP>(raw.v[x >> 2][x & 3]); }, raw.p, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
+      if (!kv4_about_middle<TP>() && ++walked % KV4_FOLD == 0) fold(lane >> 4);
       raw = nxt; b = bn; id = idn; bn = bm; idn = idm;
     }
   }
@@ -653,7 +677,7 @@ struct Kv4Sums {
 #pragma unroll
       for (int i = 0; i < HD / 32; i++) par[i] = par_next[i];
     };
-    int b = past(b0), id = kv4_page_id(a, seq, b, b1), cur = 0;
+    int b = past(b0), id = kv4_page_id(a, seq, b, b1), cur = 0, walked = 0;
     if (b >= b1) return;
     if (id >= 0) { load(id, b); make(so); }
     int bn = past(b + 1), idn = kv4_page_id(a, seq, bn, b1);
@@ -664,6 +688,7 @@ struct Kv4Sums {
       const bf16x8_t* from = so + cur * ONE + lane;
       if (id >= 0 && mine && (!MASK || b * KV4_BLK <= until))
         block<MASK>([&](int x) { return from[x * 64]; }, [&](int x) { return from[(CT + x) * 64]; }, par, b * KV4_BLK, a.window, a.scale_log2, a.gap, sp, lane);
+      if (!kv4_about_middle<TP>() && ++walked % KV4_FOLD == 0) fold(lane >> 4);
       cur ^= 1;
       if (idn >= 0) make(so + cur * ONE);
       if (idm >= 0) load(idm, bm);
@@ -674,20 +699,9 @@ struct Kv4Sums {
 
   // o becomes the columns' sums, l their denominators (over the four quarters)
   __device__ __forceinline__ void finish(int q4) {
+    fold(q4);
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      l[t] = kv4_sum_quarters(l[t]);
-#pragma unroll
-      for (int g = 0; g < G; g++) {
-        const float lg = kv4_sum_quarters(lov[t][g]);
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float add = __shfl(lg, 4 * q4 + r, 64);
-#pragma unroll
-          for (int c = 0; c < 4; c++) o[t][4 * g + c][r] += add;
-        }
-      }
-    }
+    for (int t = 0; t < NT; t++) l[t] = kv4_sum_quarters(l[t]);
   }
 };
 
@@ -925,8 +939,29 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
   }
 #pragma unroll
   for (int c = 0; c < CT; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // a head's sum over the lanes that hold its tokens
+  auto over_tokens = [&](float v) {
+    v = row_group_sum<16>(v);
+    u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    v = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false)); v = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
+    return v;
+  };
+  // the part of the los joins o: rows 0 .. RPT - 1 of the sums are in quarter(s) 0 (and 1), as this lane's heads there
+  auto fold = [&] {
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const float t = over_tokens(lov[g][r]);
+        lov[g][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[4 * g + c][r] += t;
+      }
+  };
   const int w_at = (tile >> 1) * 32 + (n16 >> 2) * 8 + 2 * (n16 & 3) + (tile & 1);      // this lane's token among a head's weights
   const float scale = a.scale_log2, gap = a.gap;
+  int steps = 0;
 
   // Steps: NB blocks each; what is not seen (or there) has levels of zero and a score of -inf.  The next step's keys are asked for when this one's are products, its values behind
   // P V, the page of the step behind in front of both: one set of registers, and no branch around the sums.
@@ -1044,25 +1079,11 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args
     }
     if (id1 >= 0) load_values(id1, b + STEP);
     id0 = id1; id1 = id2;
+    if (!kv4_about_middle<TP>() && ++steps % (KV4_FOLD / NB) == 0) fold();
   }
-  // rows 0 .. RPT - 1 of the sums are in quarter(s) 0 (and 1), as this lane's heads there
+  fold();
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    float t = row_group_sum<16>(l[r]);
-    u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false));
-    t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
-    if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false)); t = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
-    l[r] = t;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      t = row_group_sum<16>(lov[g][r]);
-      w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false));
-      t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
-      if constexpr (RPT == 4) { w = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false)); t = __uint_as_float(w[0]) + __uint_as_float(w[1]); }
-#pragma unroll
-      for (int c = 0; c < 4; c++) o[4 * g + c][r] += t;
-    }
-  }
+  for (int r = 0; r < 4; r++) l[r] = over_tokens(l[r]);
   const int nv = a.group;
   if (q4 < RPT / 4) {
 #pragma unroll
