@@ -25,7 +25,8 @@ class Held:
 
 
 def weights(q, k, head, pos, window, scale, seen=None):
-    """p [heads of one][n] of a token's queries q [heads of one][D] over key head `head`, and the score sizes: of every group the lo's and the codes' part as they come out, |scale| times their sum"""
+    """p [heads of one][n] of a token's queries q [heads of one][D] over key head `head`, and the score sizes: |scale| times, of every group, the lo's and the codes' part as they come out and, for what
+    the codes' sum is on the way, the root of its terms' squares"""
     n = len(k.x)
     j = np.arange(n)
     see = (j <= pos) & ((j > pos - window) if window else True)
@@ -35,7 +36,7 @@ def weights(q, k, head, pos, window, scale, seen=None):
     size = np.zeros(s.shape)
     for g in range(q.shape[-1] // 64):
         c = slice(64 * g, 64 * g + 64)
-        size += np.abs(q[:, c].sum(-1)[:, None] * np.where(see, k.lo[:, head, g], 0)) + np.abs(q[:, c] @ k.n[:, head, c].T) * np.where(see, k.step[:, head, g], 0)
+        size += np.abs(q[:, c].sum(-1)[:, None] * np.where(see, k.lo[:, head, g], 0)) + (np.abs(q[:, c] @ k.n[:, head, c].T) + np.sqrt(q[:, c] ** 2 @ (k.n[:, head, c] ** 2).T)) * np.where(see, k.step[:, head, g], 0)
     m = s.max(-1, keepdims=True)
     p = np.exp(s - np.where(np.isfinite(m), m, 0))
     return p / np.maximum(p.sum(-1, keepdims=True), 1e-300), abs(scale) * size
@@ -55,6 +56,27 @@ def attend(q, k, v, pos, window=0, scale=None, seen=None):
             out[t, hs] = p @ np.where((p > 0).any(0)[:, None], v.x[:, h], 0)
             size[t, hs] = np.sqrt((p * s * s).sum(-1))
     return out, size
+
+
+def inputs(lens, kv_heads, hd, dtype, seed, scale=1.0):
+    """keys and values [tokens of all sequences][kv_heads][hd] as the operators' tests take them: keys off zero by a channel's own, numbers of the storage type"""
+    rng = np.random.default_rng(seed)
+    off = 0.7 * rng.normal(size=(kv_heads, hd))
+    k = scale * (rng.normal(size=(sum(lens), kv_heads, hd)) + off)
+    v = scale * rng.normal(size=(sum(lens), kv_heads, hd))
+    return tuple(rounded(x.astype(np.float32).astype(np.float64), dtype).astype(np.float32) for x in (k, v))
+
+
+def queries(tokens, heads, hd, dtype, seed, scale=1.0):
+    return rounded((scale * np.random.default_rng(seed).normal(size=(tokens, heads, hd))).astype(np.float32).astype(np.float64), dtype).astype(np.float32)
+
+
+# (lengths, query heads a key / value head, key / value heads): a token of each sequence.  Behind `|` of the comment: walks that are divided between workgroups
+TOKENS = [([1], 4, 1), ([2, 1, 33], 4, 1), ([127, 128, 129, 130], 1, 1), ([713], 4, 1), ([300, 5, 1000], 7, 1), ([64, 700], 16, 1), ([257, 31], 2, 1), ([513, 90], 3, 5), ([90, 400], 9, 2),
+          ([3000], 4, 2), ([2100, 40], 8, 1), ([2500], 12, 1)]      # | the last line
+# (lengths, tokens brought, query heads a key / value head), two key / value heads: few columns (16, 32) and more
+PORTIONS = [([5], [5], 4), ([40, 3, 260], [2, 3, 5], 4), ([130, 700], [9, 8], 1), ([300], [300], 1), ([290, 33, 129], [70, 33, 1], 4), ([1000], [150], 7), ([200, 64], [17, 30], 16),
+            ([2600], [3], 4), ([2200, 70], [7, 5], 4), ([3000], [40], 4)]      # | the last line
 
 
 def own(size, keys, dtype):
