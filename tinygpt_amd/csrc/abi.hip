@@ -245,7 +245,7 @@ static void update_attn_modes(tgx_ctx* c, int n_positions, int rows_per_launch =
   const long long direct_lim = direct_limit(c, rpl, step), nw4_lim = nw4_limit(c, rpl, step);
   c->attn_direct = c->past + n_positions <= direct_lim;
   c->attn_nw4 = c->attn_direct && nw4_lim > 0 && c->past + n_positions <= nw4_lim;
-  c->kv4_keys = kv4_bucket(c->past + n_positions);
+  c->kv4_keys = tgx::kv4_bucket(c->past + n_positions);
   c->attn_mfma = !c->attn_direct && c->past >= attn_mfma_threshold(c) && c->dt != tgx::DT_F32 && !(c->d.qk_norm && c->d.head_dim == 128 && c->qk_fuse);
 }
 
@@ -461,7 +461,7 @@ static int run_decode_steps(tgx_ctx* c, const tgx_sampler_cfg& cfg, uint64_t see
   int remaining = n;
   while (remaining > 0) {
     int m = remaining;
-    const long long lims[3] = {nw4_limit(c, c->batch, true), direct_limit(c, c->batch, true), c->kv4 ? kv4_bucket(c->past + 1) : 0};
+    const long long lims[3] = {nw4_limit(c, c->batch, true), direct_limit(c, c->batch, true), c->kv4 ? tgx::kv4_bucket(c->past + 1) : 0};
     for (long long lim : lims)
       if (lim > 0 && c->past + 1 <= lim && c->past + m > lim) m = (int)(lim - c->past);
     update_attn_modes(c, m);

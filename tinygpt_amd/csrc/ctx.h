@@ -373,7 +373,6 @@ void kv4_launch_read(const tgx::Kv4Args& a, int hd, hipStream_t s);
 void kv4_launch_attend(tgx::Kv4Args a, const tgx::Kv4Plan& p, int hd, float* ws, hipStream_t s);
 void launch_copy_pages(const tgx::CopyPagesArgs& a, int layers, hipStream_t s);
 // a context's cache in 4 bits
-inline int kv4_bucket(long long keys) { int b = 256; while (b < keys && b < (1 << 30)) b *= 2; return b; }
 int kv4_alloc(tgx_ctx* c);                                              // pools, tables and workspace (tgx_finalize)
 int kv4_prompt_begin(tgx_ctx* c, int row0, int NB, int S);              // rows [row0, row0 + NB) write their prompts of S tokens to staging blocks ...
 void kv4_prompt_append(tgx_ctx* c, int l, int row0, int NB, int S);     // ... from which layer l's keys and values go to their pages ...

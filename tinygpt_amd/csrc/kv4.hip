@@ -176,18 +176,6 @@ tgx::Kv4Args layer_args(const tgx_ctx* c, int l, const int* tbl, int rows) {
   return a;
 }
 
-// the workspace of the steps of up to R rows
-size_t step_floats(const tgx_ctx* c) {
-  size_t need = 0;
-  for (int R = 1; R <= std::max(4, c->d.max_batch); R++)
-    for (long long keys = 256;; keys *= 2) {
-      const tgx::Kv4Plan p = tgx::kv4_plan(R, 1, c->d.kv_heads, c->d.heads / c->d.kv_heads, c->d.head_dim, 0, keys, c->num_cus);
-      need = std::max(need, tgx::kv4_part_floats(p, (long long)R * c->d.heads, c->d.head_dim));
-      if (keys >= c->d.max_ctx) break;
-    }
-  return need;
-}
-
 }  // namespace
 
 int kv4_alloc(tgx_ctx* c) {
@@ -200,7 +188,7 @@ int kv4_alloc(tgx_ctx* c) {
   HIP_OK(c, hipMemset(c->kv4_zero, 0, 4));
   hipLaunchKernelGGL(stage_tbl_kernel, dim3((c->kv_tbl_stride + 255) / 256, (unsigned)B), dim3(256), 0, c->stream, c->kv4_stage_tbl, c->kv_tbl_stride, 1);
   HIP_OK(c, hipGetLastError());
-  c->kv4_ws_floats = step_floats(c);
+  c->kv4_ws_floats = tgx::kv4_step_floats(d.max_batch, d.heads, d.kv_heads, d.head_dim, d.max_ctx, c->num_cus);
   return c->kv4_ws_floats ? dev_alloc(c, &c->kv4_ws, c->kv4_ws_floats) : TGX_OK;
 }
 

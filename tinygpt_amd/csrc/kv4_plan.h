@@ -116,4 +116,17 @@ inline Kv4Plan kv4_plan(int entries, int max_count, int kv_heads, int group, int
 }
 inline size_t kv4_part_floats(const Kv4Plan& p, long long rows, int hd) { return p.splits > 1 ? (size_t)rows * p.splits * (hd + 2) : 0; }      // workspace of the splits' records
 
+// A model's steps: the keys that the work of a step over `keys` of them is divided for (a power of two, part of a captured step's identity), and the workspace that the steps of up to
+// max_batch rows (four positions of a prompt by steps) over up to max_ctx keys need
+inline int kv4_bucket(long long keys) { int b = 256; while (b < keys && b < (1 << 30)) b *= 2; return b; }
+inline size_t kv4_step_floats(int max_batch, int heads, int kv_heads, int hd, long long max_ctx, int num_cus) {
+  size_t need = 0;
+  for (int R = 1; R <= std::max(4, max_batch); R++)
+    for (long long keys = kv4_bucket(1);; keys *= 2) {
+      need = std::max(need, kv4_part_floats(kv4_plan(R, 1, kv_heads, heads / kv_heads, hd, 0, keys, num_cus), (long long)R * heads, hd));
+      if (keys >= max_ctx) break;
+    }
+  return need;
+}
+
 }  // namespace tgx
