@@ -1326,11 +1326,9 @@ int tgx_write_kv(tgx_ctx* c, int row, int layer, const float* k_in, const float*
   HIP_OK(c, hipStreamSynchronize(c->stream));
   const tgx_model_desc& d = c->d;
   const size_t hd = (size_t)d.head_dim, per_head = (size_t)d.max_ctx * hd, T = (size_t)n_rows;
+  if (c->kv4 && (!k_in || !v_in)) return set_err(c, TGX_ERR_UNSUPPORTED, "tgx_write_kv: a cache in 4 bits takes keys and values together");
   if (c->kv_paged) { int rc = kv_own_blocks(c, row, (int)((T + tgx::KV_BLOCK - 1) / tgx::KV_BLOCK)); if (rc) return rc; HIP_OK(c, hipStreamSynchronize(c->stream)); }
-  if (c->kv4) {
-    if (!k_in || !v_in) return set_err(c, TGX_ERR_UNSUPPORTED, "tgx_write_kv: a cache in 4 bits takes keys and values together");
-    return kv4_write_rows(c, row, layer, k_in, v_in, T);
-  }
+  if (c->kv4) return kv4_write_rows(c, row, layer, k_in, v_in, T);
   std::vector<unsigned char> tmp(T * hd * c->esz);
   for (int which = 0; which < 2; which++) {
     const float* in = which ? v_in : k_in;
