@@ -485,6 +485,8 @@ TGX_API int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch,
  * heads query heads, heads / kv_heads (1 .. 16) neighbours a key / value head; out has q's dtype.  A token that sees nothing (a negative position, pages without
  * tokens) gets zeros.  k, v (both or neither): keys and values of the batch's tokens, appended first: a token sees those that other entries of its sequence bring in front
  * of it (sequences that share a page which the call appends to are one sequence to it: name it in seq).  max_keys: at least the last position + 1 of every entry; it sizes the work's division, a smaller one costs time only.
+ * max_count and max_keys choose the kernel and divide the work, for all entries alike: name the largest count where it is known (16 rows of five tokens with 80 named are worked on as portions), and
+ * call for single tokens of long rows apart from portions (together, one workgroup a key / value head walks such a row).
  * workspace: tgx_kv4_attend_workspace bytes (of the same arguments; may be 0), 16-byte aligned, the call's own until the stream is past it. */
 TGX_API int64_t tgx_kv4_attend_workspace(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, int heads, int window, int64_t max_keys, int device);
 TGX_API int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* q, int heads, const tgx_kv4_rows* k, const tgx_kv4_rows* v, float scale, int window,

@@ -33,3 +33,28 @@ def test_a_refused_write_leaves_a_fork_its_shared_blocks(missing, hip):
     with pytest.raises(TgxError):
         m._check(m.be.write_kv(m._ctx, 0, 0, None if missing == "keys" else p, None if missing == "values" else p, 300))
     assert m.get_option("kv.free_tokens") == free
+
+
+# ---- operators -------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fresh", [False, True])
+def test_batches_of_more_than_65535_tokens(fresh):
+    """66 prompts of 1000 tokens with max_count left out: what the same call gives where it names 1000, and every prompt alone"""
+    from tinygpt_amd import ops
+    n, rows, kv, hd, group = 1000, 66, 1, 64, 4
+    g = torch.Generator("cuda").manual_seed(1)
+    cache = ops.Kv4Cache.empty(1, 8 * rows, kv, hd, rows, n)
+    cache.table[:] = torch.randperm(8 * rows, device="cuda", generator=g).int().view(rows, 8)
+    k, v, q = (torch.randn(rows * n, h, hd, device="cuda", generator=g).bfloat16() for h in (kv, kv, kv * group))
+    start, offsets = ints([0] * rows), ints(range(0, rows * n + 1, n))
+    if not fresh:
+        ops.kv4_append(cache, k, v, start, offsets=offsets)
+    out = ops.kv4_attend(cache, q, start, n, offsets=offsets, **(dict(k=k, v=v) if fresh else {}))
+    assert torch.equal(out, ops.kv4_attend(cache, q, start, n, offsets=offsets, max_count=n))
+    for i in (0, 40, 65):
+        s = slice(i * n, i * n + n)
+        one = ops.kv4_attend(cache, q[s], ints([0]), n, seq=ints([i]), offsets=ints([0, n]))
+        want = torch.nn.functional.softmax((q[s].double().transpose(0, 1) @ ops.kv4_read(cache, ints([0]), n, seq=ints([i]), offsets=ints([0, n]))[0].double().permute(1, 2, 0).contiguous() / 8)
+                                           .masked_fill(~torch.ones(n, n, dtype=torch.bool, device="cuda").tril(), -float("inf")), -1)
+        want = (want @ ops.kv4_read(cache, ints([0]), n, seq=ints([i]), offsets=ints([0, n]))[1].double().transpose(0, 1)).transpose(0, 1)
+        for o in (out[s], one):      # (divided or not: within the outputs' rounding)
+            assert float(((o.double() - want) ** 2).mean()) <= float((2.0 ** -8 * want).square().mean()) / 3 * 1.02

@@ -339,7 +339,6 @@ static int attend_args(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, i
   if (heads > 65535) return op_err(TGX_ERR_UNSUPPORTED, "%d query heads", heads);
   if (window < 0 || window > (1 << 30)) return op_err(TGX_ERR_INVALID, "window %d out of range", window);
   if (max_keys < 0 || max_keys > 0x7fffffff) return op_err(TGX_ERR_INVALID, "max_keys out of range");
-  if (a.max_count > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d > 65535", a.max_count);
   a.heads = heads; a.group = heads / cache->kv_heads; a.window = window;
   return TGX_OK;
 }
@@ -371,7 +370,8 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, cache->head_dim, window, max_keys, num_cus_of(device));
   const int64_t need = (int64_t)tgx::kv4_part_floats(p, a.tokens * heads, cache->head_dim) * 4;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return op_err(TGX_ERR_INVALID, "workspace: %lld bytes aligned to 16 are needed", (long long)need);
-  if (p.tiles > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
+  // (the grids' second dimension: tiles of columns, tokens whose records are joined, blocks that are appended)
+  if (p.tiles > 65535 || (p.splits > 1 && a.max_count > 65535) || (k && blocks_of(a.max_count) > 65535)) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
   kv4_launch_attend(a, p, cache->head_dim, (float*)workspace, (hipStream_t)stream);
   return launched("kv4 attention");
 }

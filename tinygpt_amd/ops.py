@@ -195,7 +195,8 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
 
     The batch's tokens are named as in kv4_append; a token at position p sees its sequence's keys at 0 .. p, with window > 0 the last `window` of them.  k, v: the tokens'
     own keys and values, which join the cache first (a token sees itself, and what other entries bring in front of it in its sequence); without them they are there already.  max_keys: at least the last position + 1 of every
-    entry, to divide the work by.  scale: head_dim ** -0.5 where not given.  A token that sees nothing gets zeros; one that no entry names stays as it was in `out` (in a
+    entry.  max_keys and max_count (the most that an entry brings; None: all tokens) choose the kernel and divide the work, for all entries alike: name the count where it is known, and attend for
+    single tokens of long rows in a call of their own, not in one with portions.  scale: head_dim ** -0.5 where not given.  A token that sees nothing gets zeros; one that no entry names stays as it was in `out` (in a
     new one it holds anything)."""
     c, (buf, at) = _calls(), _buffer()
     if q.dim() != 3:
