@@ -58,3 +58,29 @@ def test_batches_of_more_than_65535_tokens(fresh):
         want = (want @ ops.kv4_read(cache, ints([0]), n, seq=ints([i]), offsets=ints([0, n]))[1].double().transpose(0, 1)).transpose(0, 1)
         for o in (out[s], one):      # (divided or not: within the outputs' rounding)
             assert float(((o.double() - want) ** 2).mean()) <= float((2.0 ** -8 * want).square().mean()) / 3 * 1.02
+
+
+def test_nothing_to_bring_and_nowhere_to_put_it():
+    """entries without tokens, a table without pages, a pool without any: outputs of zero for what sees nothing, and no more"""
+    from tinygpt_amd import ops
+    kv, hd, heads = 2, 64, 4
+    full = ops.Kv4Cache.empty(1, 3, kv, hd, 2, 300)
+    none, empty = torch.empty(0, kv, hd, device="cuda"), torch.empty(0, heads, hd, device="cuda")
+    for e in (1, 3):
+        batch = dict(offsets=ints([0] * (e + 1)), seq=ints([0] * e))
+        ops.kv4_append(full, none, none, ints([5] * e), **batch)
+        assert [t.shape for t in ops.kv4_read(full, ints([5] * e), 0, **batch)] == [none.shape] * 2
+        assert ops.kv4_attend(full, empty, ints([5] * e), 300, **batch).shape == empty.shape
+        assert ops.kv4_attend(full, empty, ints([5] * e), 300, k=none, v=none, **batch).shape == empty.shape
+    q, k = torch.randn(2, heads, hd, device="cuda"), torch.randn(2, kv, hd, device="cuda")
+    pool = torch.empty(1, 0, kv * hd * 144, dtype=torch.uint8, device="cuda")
+    for cache in (ops.Kv4Cache.empty(1, 3, kv, hd, 2, 0), ops.Kv4Cache(pool, torch.zeros(2, 3, dtype=torch.int32, device="cuda"), kv, hd)):
+        start = ints([0, 7])
+        ops.kv4_append(cache, k, k, start)
+        assert not any(t.any() for t in ops.kv4_read(cache, start, 2))
+        assert not ops.kv4_attend(cache, q, start, 8).any() and not ops.kv4_attend(cache, q, start, 8, k=k, v=k).any()
+        assert not ops.kv4_attend(cache, q, ints([4]), 8, offsets=ints([0, 2]), k=k, v=k).any()
+    assert ops.copy_pages(pool, ints([0, 1]), ints([1, 0])) is pool
+    other = torch.full((1, 2, kv * hd * 144), 7, dtype=torch.uint8, device="cuda")
+    ops.copy_pages(pool, ints([0, 1]), ints([1, 0]), into=other)
+    assert (other == 7).all()

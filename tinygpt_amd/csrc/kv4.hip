@@ -54,7 +54,7 @@ int check_cache(const tgx_kv4_cache* c, const tgx_kv4_batch* b, tgx::Kv4Args& a)
     return op_err(TGX_ERR_INVALID, "cache: pages / seqs / table sizes out of range");
   if (b->entries < 0 || b->entries > 65535 || b->tokens < 0 || b->tokens > 0x7fffffff || b->max_count < 0) return op_err(TGX_ERR_INVALID, "batch: entries / tokens / max_count out of range");
   if (!b->offsets && b->tokens != b->entries) return op_err(TGX_ERR_INVALID, "batch: %lld tokens of %d entries without offsets", (long long)b->tokens, b->entries);
-  if (b->entries && (!c->pool || !c->table || !b->start)) return op_err(TGX_ERR_INVALID, "null argument");
+  if (b->entries && ((!c->pool && c->pages) || (!c->table && c->seqs && c->table_len) || !b->start)) return op_err(TGX_ERR_INVALID, "null argument");      // (none of nothing: a pool without pages)
   if ((uintptr_t)c->pool & 15) return op_err(TGX_ERR_INVALID, "the pool is not aligned to 16 bytes");
   a.pool = (unsigned int*)c->pool; a.pages = c->pages; a.table = c->table; a.table_stride = c->table_stride; a.table_len = c->table_len; a.seqs = c->seqs;
   a.kv_heads = c->kv_heads;
@@ -307,10 +307,9 @@ int tgx_kv4_append(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   tgx::Kv4Args a{};
   int rc;
   if ((rc = check_cache(cache, batch, a))) return rc;
-  if (!a.entries) return TGX_OK;
+  if (!a.entries || !a.max_count || !a.tokens) return TGX_OK;
   if ((rc = check_kv(k, v, a))) return rc;
   if (blocks_of(a.max_count) > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
-  if (!a.max_count || !a.tokens) return TGX_OK;
   OnDevice on(device);
   if (on.rc) return on.rc;
   kv4_launch_append(a, cache->head_dim, (hipStream_t)stream);
@@ -321,10 +320,9 @@ int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const t
   tgx::Kv4Args a{};
   int rc;
   if ((rc = check_cache(cache, batch, a))) return rc;
-  if (!a.entries) return TGX_OK;
+  if (!a.entries || !a.max_count || !a.tokens) return TGX_OK;
   if ((rc = check_kv(k, v, a))) return rc;
   if (blocks_of(a.max_count) > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
-  if (!a.max_count || !a.tokens) return TGX_OK;
   OnDevice on(device);
   if (on.rc) return on.rc;
   kv4_launch_read(a, cache->head_dim, (hipStream_t)stream);
@@ -356,7 +354,7 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   tgx::Kv4Args a{};
   int rc;
   if ((rc = attend_args(cache, batch, heads, window, max_keys, a))) return rc;
-  if (!a.entries) return TGX_OK;
+  if (!a.entries || !a.max_count || !a.tokens) return TGX_OK;
   if ((rc = check_rows(q, "q")) || (rc = check_rows(out, "out"))) return rc;
   if (q->dtype != out->dtype) return op_err(TGX_ERR_INVALID, "q and out have different dtypes");
   if (!k != !v) return op_err(TGX_ERR_INVALID, "k and v come together");
@@ -364,7 +362,6 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   if (!std::isfinite(scale)) return op_err(TGX_ERR_INVALID, "scale is not finite");
   a.q = q->data; a.out = out->data; a.q_dt = kv4_dt(q->dtype); a.q_ts = q->token_stride; a.q_hs = q->head_stride; a.o_ts = out->token_stride; a.o_hs = out->head_stride;
   tgx::kv4_scale(a, scale);
-  if (!a.max_count || !a.tokens) return TGX_OK;
   OnDevice on(device);
   if (on.rc) return on.rc;
   const tgx::Kv4Plan p = tgx::kv4_plan(a.entries, a.max_count, a.kv_heads, a.group, cache->head_dim, window, max_keys, num_cus_of(device));
@@ -380,7 +377,7 @@ int tgx_copy_pages(const void* src, int64_t src_pages, int64_t src_stride, void*
                    const int32_t* to, int n, int device, void* stream) {
   if (n < 0 || n > 65535 || layers < 0 || layers > 65535) return op_err(TGX_ERR_INVALID, "%d pairs, %d layers (0 .. 65535)", n, layers);
   if (src_pages < 0 || dst_pages < 0 || page_bytes < 0 || src_stride < 0 || dst_stride < 0) return op_err(TGX_ERR_INVALID, "sizes out of range");
-  if (!n || !layers || !page_bytes) return TGX_OK;
+  if (!n || !layers || !page_bytes || !src_pages || !dst_pages) return TGX_OK;
   if (!src || !dst || !from || !to) return op_err(TGX_ERR_INVALID, "null argument");
   if (page_bytes % 16 || src_stride % 16 || dst_stride % 16 || ((uintptr_t)src & 15) || ((uintptr_t)dst & 15)) return op_err(TGX_ERR_INVALID, "pools, strides and pages are multiples of 16 bytes");
   if ((page_bytes + tgx::COPY_PIECE - 1) / tgx::COPY_PIECE > 0x7fffffff) return op_err(TGX_ERR_INVALID, "sizes out of range");
