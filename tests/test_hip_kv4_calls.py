@@ -6,7 +6,7 @@ import pytest
 import torch   # here, not in a test: before any module's test loads the library, which then shares torch's HIP runtime
 
 from test_hip_kv4_model import ids, make
-from tinygpt_amd.ffi import GREEDY, TgxError
+from tinygpt_amd.ffi import GREEDY, SamplerCfg, TgxError
 
 pytestmark = pytest.mark.gpu
 
@@ -33,6 +33,28 @@ def test_a_refused_write_leaves_a_fork_its_shared_blocks(missing, hip):
     with pytest.raises(TgxError):
         m._check(m.be.write_kv(m._ctx, 0, 0, None if missing == "keys" else p, None if missing == "values" else p, 300))
     assert m.get_option("kv.free_tokens") == free
+
+
+@pytest.mark.parametrize("sampler", ["greedy", "sampled"])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("grow", ["fork", "prompt"])
+def test_a_pending_token_is_fetched_behind_a_larger_batch(grow, bits, sampler, hip):
+    """steps are issued, a row joins the batch, and then their tokens are fetched: those of the same steps without it"""
+    cfg = GREEDY if sampler == "greedy" else SamplerCfg(temperature=2.0, top_p=1.0)
+    got = []
+    for joined in (False, True):
+        m, _ = make("llama_tiny", hip, "bf16", bits, max_batch=3, budget=2048)
+        p = ids(np.random.default_rng(1), 60, m.desc.vocab)[0]
+        m.forward_row(0, p)
+        m.sample_row(0, cfg, seed=3)
+        tickets = [m.step_async(cfg, seed=3) for _ in range(5)]
+        if joined:
+            if grow == "fork":
+                m.fork_row(0, 1)
+            else:
+                m.forward_row(1, p[:20])
+        got.append([m.fetch_token(t) for t in tickets])
+    assert got[0] == got[1] and len(set(got[0])) > 1
 
 
 # ---- operators -------------------------------------------------------------------------------------------------------------------------------------------

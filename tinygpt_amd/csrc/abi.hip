@@ -993,7 +993,7 @@ int tgx_fetch_token(tgx_ctx* c, int64_t ticket, int32_t* out_id) {
   if (ticket < 0 || ticket > c->steps_issued || c->steps_issued - ticket >= MAX_TICKET_EVENTS)
     return set_err(c, TGX_ERR_INVALID, "ticket %lld is not outstanding", (long long)ticket);
   HIP_OK(c, hipEventSynchronize(c->ticket_ev[ticket % MAX_TICKET_EVENTS]));
-  *out_id = c->host_ring[((ticket - 1) % HOST_RING) * c->batch];   // row 0 of the step that ticket names
+  *out_id = c->host_ring[((ticket - 1) % HOST_RING) * c->d.max_batch];   // row 0 of the step that ticket names
   return TGX_OK;
 }
 

@@ -120,7 +120,7 @@ struct tgx_ctx {
   int* step_done = nullptr;   // device: rows of the current step that have read `step` (batches; 0 between steps)
   int* tok_log = nullptr; // device ring [log_cap][rows]
   int log_cap = 0;
-  int* host_ring = nullptr;  // pinned host ring [HOST_RING][rows]
+  int* host_ring = nullptr;  // pinned host ring [HOST_RING][max_batch]
   int* host_ring_dev = nullptr;
   // pinned halves that results pass through on their way to the caller's memory (copy_to_host; allocated by its first call)
   char* stage = nullptr;

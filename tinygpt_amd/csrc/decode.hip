@@ -274,7 +274,7 @@ tgx::FinalizeArgs make_finalize_args(tgx_ctx* c, int row, bool advance_pos, bool
   tgx::FinalizeArgs a{};
   a.part_val = r.part_val; a.part_idx = r.part_idx; a.n_part = c->lm_grid;
   a.tok = r.tok; a.pos = r.pos; a.step = c->step; a.tok_log = c->tok_log; a.host_ring = c->mirror_to_host ? c->host_ring_dev : nullptr;
-  a.log_cap = c->log_cap; a.ring_cap = HOST_RING;
+  a.log_cap = c->log_cap; a.ring_cap = HOST_RING; a.ring_rows = c->d.max_batch;
   a.row = row; a.rows = c->batch;
   a.log = log_step ? 1 : 0; a.bump_step = (row == c->batch - 1) ? 1 : 0;
   if (log_step && c->batch > 1) { a.done = c->step_done; a.done_total = c->batch; a.bump_step = 0; }      // rows of a batch may be finalized concurrently: the last to count itself moves the step

@@ -64,8 +64,9 @@ struct FinalizeArgs {
   int* pos;              // this row's pastLength
   int* step;             // decode steps finalized so far (monotonic; index into the token rings)
   int* tok_log;          // [log_cap][rows] device ring of produced tokens
-  volatile int* host_ring;   // [ring_cap][rows] pinned host mirror (AsyncTokenPipeline read-back); nullptr: not mirrored (multi-step graphs)
+  volatile int* host_ring;   // [ring_cap][ring_rows] pinned host mirror (AsyncTokenPipeline read-back); nullptr: not mirrored (multi-step graphs)
   int log_cap, ring_cap;
+  int ring_rows;         // the context's rows, however many a step has: a step's place does not depend on the batch at the time its token is fetched
   int row, rows;
   int log;               // 1: record the token in the rings (decode steps); 0: tgx_sample after a prefill
   int bump_step;         // 1 on the last row of a step (batch 1, or rows finalized by consecutive launches)
@@ -90,7 +91,7 @@ __device__ __forceinline__ void publish_token(const FinalizeArgs& a, int best, i
   if (a.log) {
     const int st = *a.step;
     a.tok_log[(st % a.log_cap) * a.rows + a.row] = t;
-    if (a.host_ring) a.host_ring[(st % a.ring_cap) * a.rows + a.row] = t;
+    if (a.host_ring) a.host_ring[(st % a.ring_cap) * a.ring_rows + a.row] = t;
     if (a.done) { if (atomicAdd(a.done, 1) == a.done_total - 1) { *a.done = 0; *a.step = st + 1; } }
     else if (a.bump_step) *a.step = st + 1;
   }

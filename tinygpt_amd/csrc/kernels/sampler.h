@@ -487,7 +487,7 @@ __device__ __forceinline__ void samp_draw_and_publish(const SampArgs& a, const F
     if (fin.log) {
       const int st = dw.step;
       fin.tok_log[(st % fin.log_cap) * fin.rows + fin.row] = pick;
-      if (fin.host_ring) fin.host_ring[(st % fin.ring_cap) * fin.rows + fin.row] = pick;
+      if (fin.host_ring) fin.host_ring[(st % fin.ring_cap) * fin.ring_rows + fin.row] = pick;
       if (fin.done) { if (atomicAdd(fin.done, 1) == fin.done_total - 1) { *fin.done = 0; *fin.step = st + 1; } }
       else if (fin.bump_step) *fin.step = st + 1;
     }
