@@ -106,3 +106,16 @@ def test_nothing_to_bring_and_nowhere_to_put_it():
     other = torch.full((1, 2, kv * hd * 144), 7, dtype=torch.uint8, device="cuda")
     ops.copy_pages(pool, ints([0, 1]), ints([1, 0]), into=other)
     assert (other == 7).all()
+
+
+def test_a_generation_finds_its_workspace_again():
+    """max_keys grows with every token: the workspace's size is asked of the library once a page of 128"""
+    from tinygpt_amd import ops
+    cache = ops.Kv4Cache.empty(1, 40, 2, 64, 1, 5000)
+    cache.table[0] = torch.arange(cache.table.shape[1], device="cuda").int()
+    q, k = torch.randn(1, 8, 64, device="cuda"), torch.randn(1, 2, 64, device="cuda")
+    for keys in range(1, 641):
+        ops.kv4_attend(cache, q, ints([keys - 1]), keys, k=k, v=k)
+        if keys == 1:
+            misses = ops._workspace.cache_info().misses
+    assert ops._workspace.cache_info().misses - misses <= 4

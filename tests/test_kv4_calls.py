@@ -33,3 +33,22 @@ def test_batches_without_tokens_need_no_buffers(be, name):  # noqa: F811
 def test_copies_of_pools_without_pages(be):  # noqa: F811
     for src, dst in [(0, 4), (4, 0), (0, 0)]:
         assert be.copy_pages(4096 if src else None, src, 4096, 8192 if dst else None, dst, 4096, 2, 256, 4096, 4096, 2, 0, None) == 0
+
+
+@pytest.mark.parametrize("window", [0, 100, 5000])
+@pytest.mark.parametrize("max_count,entries,heads", [(1, 1, 8), (1, 32, 8), (5, 3, 4), (300, 1, 8)])
+def test_the_keys_of_a_page_need_one_workspace(be, max_count, entries, heads, window):  # noqa: F811
+    """ops.kv4_attend looks a workspace up by whole pages of max_keys: what the library says for max_keys itself"""
+    from tinygpt_amd.ops import _whole_pages
+    needs = set()
+    for keys in [0, 1, 2, 127, 128, 129, 255, 256, 257, 700, 1023, 1024, 1025, 4095, 4097, 30000, 131071, 131072, 2 ** 31 - 129, 2 ** 31 - 128, 2 ** 31 - 127, 2 ** 31 - 1]:
+        size = dict(entries=entries, seqs=entries, tokens=entries * max_count, max_count=max_count, offsets=4096, heads=heads, window=window)
+        needs.add(attend(be, keys=keys, **size))
+        assert attend(be, keys=keys, **size) == attend(be, keys=_whole_pages(keys), **size) >= 0, keys
+    assert len(needs) > 1 or window or max_count == 300
+
+
+def test_a_generation_looks_its_workspace_up_once_a_page():
+    from tinygpt_amd.ops import _whole_pages
+    assert len({_whole_pages(k) for k in range(1, 1025)}) == 8
+    assert _whole_pages(0) == 0 and _whole_pages(-1) == 0 and _whole_pages(2 ** 40) == 2 ** 31 - 1

@@ -77,6 +77,11 @@ def _workspace(entries, max_count, tokens, kv_heads, head_dim, heads, window, ma
     return max(0, _calls().kv4_attend_workspace(ctypes.cast(cache, ctypes.c_void_p), ctypes.cast(batch, ctypes.c_void_p), heads, window, max_keys, device))
 
 
+def _whole_pages(max_keys):
+    """the keys by which work is divided: pages of them count, so that a row's workspace is looked up anew once a page and not with every token"""
+    return min(-(-max_keys // PAGE_TOKENS) * PAGE_TOKENS, 2 ** 31 - 1)
+
+
 def kv4_page_bytes(kv_heads: int, head_dim: int) -> int:
     """bytes of a page (128 tokens of all key / value heads of a layer)"""
     n = product_backend().kv4_page_bytes(kv_heads, head_dim)
@@ -216,7 +221,7 @@ def kv4_attend(cache: Kv4Cache, q: torch.Tensor, start: torch.Tensor, max_keys: 
         _pack_rows(buf, _AT_V, "v", v, tokens, cache.kv_heads, cache)
     cache._pack(buf, layer)
     index = cache.index
-    need = _workspace(entries, max_count, tokens, cache.kv_heads, cache.head_dim, heads, window, max_keys, index)
+    need = _workspace(entries, max_count, tokens, cache.kv_heads, cache.head_dim, heads, window, _whole_pages(max_keys), index)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     c.check(c.kv4_attend(at + _AT_CACHE, at + _AT_BATCH, at + _AT_Q, heads, None if k is None else at + _AT_K, None if k is None else at + _AT_V, cache.head_dim ** -0.5 if scale is None else scale,
                          window, max_keys, at + _AT_OUT, ws.data_ptr() if need else None, need, index, _stream(index)))
