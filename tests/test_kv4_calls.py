@@ -1,6 +1,10 @@
 """Calls of the 4-bit operators that are not refused, and what they need, on the CPU."""
+import os
+import re
+
 import pytest
 
+from conftest import ROOT
 from test_kv4_plan import be, call  # noqa: F401  (be: a fixture)
 
 
@@ -52,3 +56,10 @@ def test_a_generation_looks_its_workspace_up_once_a_page():
     from tinygpt_amd.ops import _whole_pages
     assert len({_whole_pages(k) for k in range(1, 1025)}) == 8
     assert _whole_pages(0) == 0 and _whole_pages(-1) == 0 and _whole_pages(2 ** 40) == 2 ** 31 - 1
+
+
+def test_bytes_in_lds_are_aligned_for_wider_reads():
+    """arrays of bytes that a kernel of kv4.h holds in LDS are read as words: each says its alignment"""
+    with open(os.path.join(ROOT, "tinygpt_amd", "csrc", "kernels", "kv4.h")) as f:
+        arrays = re.findall(r"^.*__shared__.*unsigned char .*$", f.read(), re.M)
+    assert len(arrays) == 2 and all("aligned(16)" in a for a in arrays), arrays

@@ -208,7 +208,7 @@ __global__ __launch_bounds__(2 * HD) void kv4_append_block_kernel(const Kv4Args 
 template <int HD, int DT>
 __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
   constexpr int PARTS = HD / 64;
-  __shared__ unsigned char s[KV4_BLK * (HD + 8)];
+  __shared__ __attribute__((aligned(16))) unsigned char s[KV4_BLK * (HD + 8)];      // (eight bytes at a time below)
   const Kv4Entry en = kv4_entry(a, blockIdx.z);
   const int kvh = blockIdx.x, lane = threadIdx.x, q = lane >> 4, r = lane & 15;
   if (en.count < 1) return;
