@@ -465,7 +465,7 @@ typedef struct tgx_kv4_batch {
   const int32_t* offsets;
 } tgx_kv4_batch;
 
-/* [tokens][heads][head_dim] on the device: strides in elements, a head's channels lie together */
+/* [tokens][heads][head_dim] on the device: strides in elements, a head's channels lie together; in an output every token and head has a place of its own */
 typedef struct tgx_kv4_rows {
   void* data;
   int32_t dtype;         /* tgx_dtype */

@@ -119,3 +119,20 @@ def test_a_generation_finds_its_workspace_again():
         if keys == 1:
             misses = ops._workspace.cache_info().misses
     assert ops._workspace.cache_info().misses - misses <= 4
+
+
+def test_outputs_that_lie_on_each_other_are_refused():
+    from tinygpt_amd import ops
+    cache = ops.Kv4Cache.empty(1, 4, 2, 64, 2, 300)
+    cache.table[:] = ints(range(4)).view(2, 2).repeat(1, 2)[:, :cache.table.shape[1]]
+    q, start = torch.randn(2, 4, 64, device="cuda"), ints([0, 5])
+    k = torch.randn(1, 2, 64, device="cuda").expand(2, 2, 64)      # the same token twice: an input may
+    ops.kv4_append(cache, k, k, start)
+    for shape in [(1, 4, 64), (2, 1, 64), (1, 1, 64)]:
+        with pytest.raises(TgxError):
+            ops.kv4_attend(cache, q, start, 300, out=torch.zeros(shape, device="cuda").expand(2, 4, 64))
+    with pytest.raises(TgxError):
+        ops.kv4_read(cache, start, 2, out=(torch.zeros(2, 2, 64, device="cuda"), torch.zeros(1, 2, 64, device="cuda").expand(2, 2, 64)))
+    one = torch.zeros(1, 4, 64, device="cuda")
+    ops.kv4_attend(cache, q[:1], start[:1], 300, out=one.as_strided((1, 4, 64), (0, 64, 1)))      # one token: its stride says nothing
+    assert torch.equal(one, ops.kv4_attend(cache, q[:1], start[:1], 300)) and one.any()

@@ -63,3 +63,15 @@ def test_bytes_in_lds_are_aligned_for_wider_reads():
     with open(os.path.join(ROOT, "tinygpt_amd", "csrc", "kernels", "kv4.h")) as f:
         arrays = re.findall(r"^.*__shared__.*unsigned char .*$", f.read(), re.M)
     assert len(arrays) == 2 and all("aligned(16)" in a for a in arrays), arrays
+
+
+def test_outputs_that_lie_on_each_other_are_refused(be):  # noqa: F811
+    """a stride of 0 in an output of several tokens or heads; inputs may repeat"""
+    from tinygpt_amd.ffi import Kv4BatchArg, Kv4CacheArg, Kv4RowsArg
+    c, b = Kv4CacheArg(4096, 4, 4096, 3, 3, 2, 2, 64), Kv4BatchArg(2, 1, 2, None, 4096, None)
+    good = Kv4RowsArg(4096, 1, 256, 64)
+    for token, head in [(0, 64), (256, 0), (0, 0)]:
+        bad = Kv4RowsArg(4096, 1, token, head)
+        assert be.kv4_read(c, b, bad, good, 0, None) == 1 and be.kv4_read(c, b, good, bad, 0, None) == 1
+        assert be.kv4_attend(c, b, good, 4, good, good, 0.125, 0, 300, bad, 4096, 1 << 40, 0, None) == 1
+        assert b"share memory" in be.op_last_error()

@@ -78,6 +78,12 @@ int check_kv(const tgx_kv4_rows* k, const tgx_kv4_rows* v, tgx::Kv4Args& a) {
   return TGX_OK;
 }
 
+// outputs whose tokens or heads lie on each other would hold whichever was written last
+int check_apart(const tgx_kv4_rows* r, const char* name, int64_t tokens, int heads) {
+  if ((tokens > 1 && !r->token_stride) || (heads > 1 && !r->head_stride)) return op_err(TGX_ERR_INVALID, "%s: tokens or heads share memory (a stride of 0)", name);
+  return TGX_OK;
+}
+
 // blocks of 32 positions that an entry of n tokens may touch
 int blocks_of(int n) { return (n + 30) / 32 + 1; }
 
@@ -321,7 +327,7 @@ int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const t
   int rc;
   if ((rc = check_cache(cache, batch, a))) return rc;
   if (!a.entries || !a.max_count || !a.tokens) return TGX_OK;
-  if ((rc = check_kv(k, v, a))) return rc;
+  if ((rc = check_kv(k, v, a)) || (rc = check_apart(k, "k", a.tokens, a.kv_heads)) || (rc = check_apart(v, "v", a.tokens, a.kv_heads))) return rc;
   if (blocks_of(a.max_count) > 65535) return op_err(TGX_ERR_UNSUPPORTED, "max_count %d", a.max_count);
   OnDevice on(device);
   if (on.rc) return on.rc;
@@ -355,7 +361,7 @@ int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const
   int rc;
   if ((rc = attend_args(cache, batch, heads, window, max_keys, a))) return rc;
   if (!a.entries || !a.max_count || !a.tokens) return TGX_OK;
-  if ((rc = check_rows(q, "q")) || (rc = check_rows(out, "out"))) return rc;
+  if ((rc = check_rows(q, "q")) || (rc = check_rows(out, "out")) || (rc = check_apart(out, "out", a.tokens, heads))) return rc;
   if (q->dtype != out->dtype) return op_err(TGX_ERR_INVALID, "q and out have different dtypes");
   if (!k != !v) return op_err(TGX_ERR_INVALID, "k and v come together");
   if (k && (rc = check_kv(k, v, a))) return rc;
