@@ -32,7 +32,9 @@ extern "C" {
                              * 7: Zaluvik (layer norms around every sublayer, a looped span of layers, un-normalised sigmoid attention with mixed heads,
                              *    windowed latent attention with a shared rotated key part, sigmoid group-limited router);
                              * 8: Nusovik (norms on the sublayers' outputs only, two state-space mixers, bucketed distance bias, per-head sink and gate);
-                             * 9: Keronex (several residual streams, pair embedding, retention, channel-decay delta rule, two-map attention, layers that share weights) */
+                             * 9: Keronex (several residual streams, pair embedding, retention, channel-decay delta rule, two-map attention, layers that share weights).
+                             * It moves when a struct or a call that was there changes.  tgx_fork_row, tgx_resize_kv, tgx_kv4_*, tgx_copy_pages and tgx_op_last_error joined version 9: a host
+                             * that may meet a library without them looks the symbols up */
 
 #if defined(__GNUC__)
 #define TGX_API __attribute__((visibility("default")))
@@ -478,7 +480,7 @@ TGX_API int64_t tgx_kv4_page_bytes(int kv_heads, int head_dim);      /* -1: not 
 /* Keys and values of the batch's tokens into their pages (k and v of one dtype); a token with a negative position is left out.  The rest of a page stays as it is. */
 TGX_API int tgx_kv4_append(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream);
 
-/* The values that the pages hold for the batch's tokens, each rounded once to the dtype of k and v. */
+/* The values that the pages hold for the batch's tokens, each rounded once to the dtype of k and v; tokens with a negative position are left as they were, those without a page read as zeros. */
 TGX_API int tgx_kv4_read(const tgx_kv4_cache* cache, const tgx_kv4_batch* batch, const tgx_kv4_rows* k, const tgx_kv4_rows* v, int device, void* stream);
 
 /* out = softmax(scale q . k) v over the keys that a token sees: those of its sequence at positions 0 .. its own, with window > 0 only the last `window` of them.

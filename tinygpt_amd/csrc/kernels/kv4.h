@@ -204,7 +204,7 @@ __global__ __launch_bounds__(2 * HD) void kv4_append_block_kernel(const Kv4Args 
 }
 
 // The values that the pages hold for the batch's tokens: a wave a (entry, block of 32 positions, kv head).  Bound by its stores, 16 bits or more for 4.5 that it reads: four rows of up to 4096
-// tokens, eight heads of 128, 14 us (3.4 TB/s); a token of each of 64 rows 4.2 us.
+// tokens, eight heads of 128, 14.4 us (4.0 TB/s); a token of each of 64 rows 3.9 us.
 template <int HD, int DT>
 __global__ __launch_bounds__(64) void kv4_read_kernel(const Kv4Args a) {
   constexpr int PARTS = HD / 64;
@@ -751,7 +751,7 @@ __device__ __forceinline__ void kv4_append_first(const Kv4Args& a, const Kv4Entr
 }
 
 // Few columns (a few tokens' query heads): the KW waves of a workgroup divide the keys, wave w the blocks w, w + KW, ... of the split's; all columns in each.
-// 16 rows of up to 2000 tokens, five tokens each, 16 / 8 heads of 128: 14 us (1.7 TB/s), a way of eight blocks a wave between its start and the meeting of the waves.
+// 16 rows of up to 2000 tokens, five tokens each, 16 / 8 heads of 128: 13 us (1.9 TB/s), a way of eight blocks a wave between its start and the meeting of the waves.
 template <int HD, int NT, int KW, int QT, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args a) {
   typedef Kv4Sums<HD, NT, QT, TQ, TP> Sums;
@@ -792,7 +792,7 @@ __global__ __launch_bounds__(64 * KW) void kv4_attend_keys_kernel(const Kv4Args 
 }
 
 // Many columns (portions): the four waves of a workgroup divide them, 16 NT each, and walk the same keys, whose operands they make together.  Bound by the vector units, some 370 instructions a
-// block of 32 tokens and 32 columns beside 52 of the matrix units: 2048 tokens behind 6144, 32 / 8 heads of 128, 476 us (505 TFLOP/s).  Operands made by each wave for itself: 30 us more;
+// block of 32 tokens and 32 columns beside 52 of the matrix units: 2048 tokens behind 6144, 32 / 8 heads of 128, 487 us with their append and read-back (495 TFLOP/s).  Operands made by each wave for itself: 30 us more;
 // tiles in their order, so that a compute unit gets two with many keys: 80 us more.
 template <int HD, int NT, int QT, int TQ, int TP>
 __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a) {
@@ -851,8 +851,8 @@ __global__ __launch_bounds__(256) void kv4_attend_columns_kernel(const Kv4Args a
 // over, so that the products of 16 / RPT tiles of tokens give every lane the scores of one token for four heads (quarter q takes its rows from the product of tile q, or q / 2): a lane
 // reads the parameters of its own token, and each score, exponential and weight is worked out once and not for 16 columns of which RPT are asked for.  The weights
 // pass through LDS into the A operand of P V (rows heads).  What a row's four heads share (references, their sums' factors) is the same in every lane that holds the row.
-// Memory and vector units overlap but for a fifth: 32 rows of up to 4096 tokens, 32 / 8 heads of 128, 24.8 us (4.1 TB/s; 19 to 21 without the arithmetic), one of 131071 with 64 / 8 heads 33.5
-// (4.5 TB/s; 25).  Short rows are one dependent way, table, page, sums: 300 tokens, 7.5 us (3.7 without the arithmetic).
+// Memory and vector units overlap but for a fifth: 32 rows of up to 4096 tokens, 32 / 8 heads of 128, 25.2 us (4.0 TB/s; 19 to 21 without the arithmetic), one of 131071 with 64 / 8 heads 34.0
+// (4.4 TB/s; 25).  Short rows are one dependent way, table, page, sums: 713 tokens, 7.1 us (3.7 without the arithmetic).
 template <int HD, int RPT, int KW, int QT, int TQ, int TP>
 __global__ __launch_bounds__(64 * KW) void kv4_attend_token_kernel(const Kv4Args a) {
   constexpr int G = HD / 64, CH = HD / 32, CT = HD / 16, PARTS = HD / 64, PW = HD / 32;
