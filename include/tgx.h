@@ -495,8 +495,8 @@ TGX_API int tgx_kv4_attend(const tgx_kv4_cache* cache, const tgx_kv4_batch* batc
                            int64_t max_keys, const tgx_kv4_rows* out, void* workspace, int64_t workspace_bytes, int device, void* stream);
 
 /* Pages between (or inside) paged pools, 4-bit or 16-bit: for every layer l and pair i, page to[i] of dst becomes page from[i] of src.  A page is page_bytes (a
- * multiple of 16), a layer's pool starts l * src_stride / dst_stride bytes (multiples of 16) behind src / dst.  from, to: device [n]; a pair with a page outside
- * of its pool is left out.  No page is read and written, or written twice, by one call. */
+ * multiple of 16), a layer's pool starts l * src_stride / dst_stride bytes (multiples of 16) behind src / dst; the layers of dst do not overlap.
+ * from, to: device [n]; a pair with a page outside of its pool is left out.  No page is read and written, or written twice, by one call. */
 TGX_API int tgx_copy_pages(const void* src, int64_t src_pages, int64_t src_stride, void* dst, int64_t dst_pages, int64_t dst_stride, int layers, int64_t page_bytes,
                            const int32_t* from, const int32_t* to, int n, int device, void* stream);
 

@@ -136,3 +136,16 @@ def test_outputs_that_lie_on_each_other_are_refused():
     one = torch.zeros(1, 4, 64, device="cuda")
     ops.kv4_attend(cache, q[:1], start[:1], 300, out=one.as_strided((1, 4, 64), (0, 64, 1)))      # one token: its stride says nothing
     assert torch.equal(one, ops.kv4_attend(cache, q[:1], start[:1], 300)) and one.any()
+
+
+def test_copies_into_layers_that_share_memory_are_refused():
+    from tinygpt_amd import ops
+    pool = torch.randint(0, 99, (1, 4, 64), device="cuda", dtype=torch.int32)
+    with pytest.raises(TgxError):
+        ops.copy_pages(torch.zeros(3, 4, 64, device="cuda", dtype=torch.int32), ints([0]), ints([1]), into=pool.expand(3, 4, 64))
+    into = torch.zeros(3, 4, 64, device="cuda", dtype=torch.int32)
+    ops.copy_pages(pool.expand(3, 4, 64), ints([2, 0]), ints([1, 3]), into=into)      # one layer into three
+    assert torch.equal(into[:, [1, 3]], pool[:, [2, 0]].expand(3, 2, 64)) and not into[:, [0, 2]].any()
+    wide = torch.zeros(3, 6, 64, device="cuda", dtype=torch.int32)                    # pages of a larger pool: layers further apart than their pages
+    ops.copy_pages(pool.expand(3, 4, 64), ints([2, 0]), ints([1, 3]), into=wide[:, 1:5])
+    assert torch.equal(wide[:, [2, 4]], pool[:, [2, 0]].expand(3, 2, 64)) and not wide[:, [0, 1, 3, 5]].any()

@@ -75,3 +75,10 @@ def test_outputs_that_lie_on_each_other_are_refused(be):  # noqa: F811
         assert be.kv4_read(c, b, bad, good, 0, None) == 1 and be.kv4_read(c, b, good, bad, 0, None) == 1
         assert be.kv4_attend(c, b, good, 4, good, good, 0.125, 0, 300, bad, 4096, 1 << 40, 0, None) == 1
         assert b"share memory" in be.op_last_error()
+
+
+def test_copies_into_layers_that_share_memory_are_refused(be):  # noqa: F811
+    """pages of one layer of the destination would be another's; a source may repeat (one layer into several)"""
+    for stride, pages, layers, status in [(0, 4, 2, 1), (256 * 3, 4, 2, 1), (256 * 4 - 16, 4, 2, 1), (256, 2, 9, 1)]:
+        assert be.copy_pages(4096, 4, 1024, 8192, pages, stride, layers, 256, 4096, 4096, 2, 0, None) == status, stride
+        assert b"share memory" in be.op_last_error()

@@ -387,6 +387,7 @@ int tgx_copy_pages(const void* src, int64_t src_pages, int64_t src_stride, void*
   if (!src || !dst || !from || !to) return op_err(TGX_ERR_INVALID, "null argument");
   if (page_bytes % 16 || src_stride % 16 || dst_stride % 16 || ((uintptr_t)src & 15) || ((uintptr_t)dst & 15)) return op_err(TGX_ERR_INVALID, "pools, strides and pages are multiples of 16 bytes");
   if ((page_bytes + tgx::COPY_PIECE - 1) / tgx::COPY_PIECE > 0x7fffffff) return op_err(TGX_ERR_INVALID, "sizes out of range");
+  if (layers > 1 && (dst_stride / page_bytes < dst_pages)) return op_err(TGX_ERR_INVALID, "dst: layers share memory (%lld bytes between them, %lld pages of %lld)", (long long)dst_stride, (long long)dst_pages, (long long)page_bytes);
   OnDevice on(device);
   if (on.rc) return on.rc;
   tgx::CopyPagesArgs a{};
