@@ -33,8 +33,8 @@ extern "C" {
                              *    windowed latent attention with a shared rotated key part, sigmoid group-limited router);
                              * 8: Nusovik (norms on the sublayers' outputs only, two state-space mixers, bucketed distance bias, per-head sink and gate);
                              * 9: Keronex (several residual streams, pair embedding, retention, channel-decay delta rule, two-map attention, layers that share weights).
-                             * It moves when a struct or a call that was there changes.  tgx_fork_row, tgx_resize_kv, tgx_kv4_*, tgx_copy_pages and tgx_op_last_error joined version 9: a host
-                             * that may meet a library without them looks the symbols up */
+                             * tgx_fork_row, tgx_resize_kv, tgx_kv4_*, tgx_copy_pages and tgx_op_last_error joined version 9 and change nothing that was there: a host that may meet a
+                             * library without them looks the symbols up */
 
 #if defined(__GNUC__)
 #define TGX_API __attribute__((visibility("default")))

@@ -149,3 +149,21 @@ def test_copies_into_layers_that_share_memory_are_refused():
     wide = torch.zeros(3, 6, 64, device="cuda", dtype=torch.int32)                    # pages of a larger pool: layers further apart than their pages
     ops.copy_pages(pool.expand(3, 4, 64), ints([2, 0]), ints([1, 3]), into=wide[:, 1:5])
     assert torch.equal(wide[:, [2, 4]], pool[:, [2, 0]].expand(3, 2, 64)) and not wide[:, [0, 1, 3, 5]].any()
+
+
+def test_a_read_of_positions_that_are_not_there():
+    """negative positions are left as they were, positions without a page read as zeros, in every type and by tokens and portions"""
+    from tinygpt_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        cache = ops.Kv4Cache.empty(1, 3, 2, 64, 1, 300)
+        cache.table[0, 0] = 2      # and no second page
+        x = torch.randn(128, 2, 64, device="cuda").to(dtype)
+        ops.kv4_append(cache, x, x, ints([0]), offsets=ints([0, 128]))
+        k, v = torch.full((2, 160, 2, 64), 7.0, dtype=dtype, device="cuda").unbind(0)
+        ops.kv4_read(cache, ints([-10]), 160, offsets=ints([0, 160]), out=(k, v))
+        for t in (k, v):
+            assert (t[:10] == 7).all() and not t[138:].any() and (t[10:138] - x).abs().max() < 0.5
+            assert torch.equal(t[10:138], ops.kv4_read(cache, ints([0]), 128, dtype=dtype, offsets=ints([0, 128]))[0])
+        one = torch.full((2, 1, 2, 64), 7.0, dtype=dtype, device="cuda")
+        ops.kv4_read(cache, ints([-1]), 1, out=one.unbind(0))
+        assert (one == 7).all()

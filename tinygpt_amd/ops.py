@@ -183,7 +183,7 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
 def kv4_read(cache: Kv4Cache, start: torch.Tensor, tokens: int, dtype: torch.dtype = torch.float32, layer: int = 0, seq: torch.Tensor = None, offsets: torch.Tensor = None,
              max_count: int = None, out=None):
     """The values that the cache holds for a batch's tokens, named as in kv4_append: (keys, values), each [tokens][kv_heads][head_dim], rounded once to dtype.
-    out: tensors to write to; tokens that no entry names stay as they were in them (in new ones they hold anything)."""
+    out: tensors to write to; tokens that no entry names or that have a negative position stay as they were in them (in new ones they hold anything), tokens without a page read as zeros."""
     c, (buf, at) = _calls(), _buffer()
     k, v = out if out is not None else torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device).unbind(0)
     _pack_batch(buf, cache, tokens, start, seq, offsets, max_count)
